@@ -390,6 +390,49 @@ SNB_API int snb_codebook_cross_entropy(void* stream, const void* logits, int32_t
                                        uint64_t targets_len, const float* grad_scales, float* loss_sums,
                                        void* logits_grad, int32_t grad_type);
 
+/* Softmax cross entropy over a large vocabulary, with its gradients, without the logits: for hidden rows h and the
+ * classes' weight rows w_v, z_v = h . w_v, losses[row] = log sum_v exp(z_v) - z_target, and with p = softmax(z) - onehot
+ *   hidden_grad[row] = grad_scale * sum_v p_v w_v,   weight_grad[v] = grad_scale * sum_rows p_v h.
+ * The vocabulary is taken in pieces: one pass over it for the rows' log-sum-exp, and for gradients a second one that
+ * computes each piece's logits again, so the logits are never held. */
+typedef struct snb_vocabulary_loss_args {
+    uint64_t rows, width, classes;
+    int32_t type;              /* SNB_TYPE_* of hidden and weight. bf16: bf16 tensor cores, p rounded to bf16 for the two
+                                * gradient products. f32: TF32 tensor cores on operands split in two, f32 accuracy. */
+    int32_t weight_transposed; /* 1: weight is [classes, width] (a tied embedding); 0: [width, classes] (a Linear) */
+    const void* hidden;        /* [rows, width], rows hidden_stride elements apart */
+    uint64_t hidden_len, hidden_stride;
+    const void* weight;        /* rows weight_stride elements apart */
+    uint64_t weight_len, weight_stride;
+    const uint32_t* targets;   /* [rows]; 0xFFFFFFFF: the row has none (loss 0, zero gradient, whatever it holds);
+                                * any other value >= classes gives a NaN loss and gradient */
+    uint64_t targets_len;
+    float* losses;             /* [rows] */
+    uint64_t losses_len;
+    float* loss_sum;           /* their sum, in a fixed order; or NULL */
+    float grad_scale;
+    int32_t flags;             /* SNB_GEMM_DETERMINISTIC: bit-identical gradients from run to run; or 0 */
+    void* hidden_grad;         /* [rows, width], overwritten; or NULL */
+    uint64_t hidden_grad_len;
+    void* weight_grad;         /* dense, in the weight's order; or NULL */
+    uint64_t weight_grad_len;
+    int32_t hidden_grad_type, weight_grad_type; /* SNB_TYPE_* (f32 for f32 operands) */
+    int32_t accumulate;        /* 1: weight_grad += (f32 only); 0: overwritten */
+    int32_t reserved;
+    void* workspace;           /* snb_vocabulary_cross_entropy_workspace bytes, used until the call's work is done */
+    uint64_t workspace_len;
+} snb_vocabulary_loss_args;
+
+/* *bytes = the workspace that a call with these arguments needs (the workspace fields are not read): statistics of
+ * rows * classes / 16 bytes; for gradients a piece of p of at most 256 MB (or 256 classes), a packed copy of hidden and
+ * f32 sums of hidden's size; and where the weight is f32 or not laid out for TMA (16-byte aligned rows), a packed piece
+ * of it of at most 256 MB. */
+SNB_API int snb_vocabulary_cross_entropy_workspace(const snb_vocabulary_loss_args* args, uint64_t* bytes);
+
+/* Needs sm_100 tensor cores (SNB_ERR_UNSUPPORTED otherwise). Checks, in this order: sizes and types, lengths, null
+ * pointers, workspace. No reference counterpart (the reference keeps the logits of its 1,024-class heads). */
+SNB_API int snb_vocabulary_cross_entropy(void* stream, const snb_vocabulary_loss_args* args);
+
 /* ---------------------------------------------------------------------------------------------- RMSNorm, AdamW */
 
 /* RMSNorm forward (`Gpu::rms_norm_forward`, ops/normalization.rs; kernel kernels/normalization.rs:27-51): for each

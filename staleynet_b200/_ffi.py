@@ -69,6 +69,8 @@ EXPORTED_SYMBOLS = (
     "snb_cross_entropy",
     "snb_head_cross_entropy",
     "snb_codebook_cross_entropy",
+    "snb_vocabulary_cross_entropy_workspace",
+    "snb_vocabulary_cross_entropy",
     "snb_split_heads",
     "snb_merge_heads",
     "snb_permute_heads",
@@ -167,6 +169,18 @@ class GemmArgs(ctypes.Structure):
     ]
 
 
+class VocabularyLossArgs(ctypes.Structure):
+    """snb_vocabulary_loss_args."""
+    _fields_ = [("rows", c_uint64), ("width", c_uint64), ("classes", c_uint64), ("type", c_int32),
+                ("weight_transposed", c_int32), ("hidden", c_void_p), ("hidden_len", c_uint64),
+                ("hidden_stride", c_uint64), ("weight", c_void_p), ("weight_len", c_uint64),
+                ("weight_stride", c_uint64), ("targets", c_void_p), ("targets_len", c_uint64), ("losses", c_void_p),
+                ("losses_len", c_uint64), ("loss_sum", c_void_p), ("grad_scale", c_float), ("flags", c_int32),
+                ("hidden_grad", c_void_p), ("hidden_grad_len", c_uint64), ("weight_grad", c_void_p),
+                ("weight_grad_len", c_uint64), ("hidden_grad_type", c_int32), ("weight_grad_type", c_int32),
+                ("accumulate", c_int32), ("reserved", c_int32), ("workspace", c_void_p), ("workspace_len", c_uint64)]
+
+
 assert ctypes.sizeof(Operand) == 24
 assert ctypes.sizeof(Product) == 88
 assert ctypes.sizeof(HeadLayout) == 64
@@ -233,6 +247,10 @@ def load() -> ctypes.CDLL:
         lib.snb_codebook_cross_entropy.argtypes = [c_void_p, c_void_p, c_int32, c_uint64, c_uint64, c_uint64,
                                                    c_void_p, c_uint64, c_void_p, c_void_p, c_void_p, c_int32]
         lib.snb_codebook_cross_entropy.restype = c_int
+        lib.snb_vocabulary_cross_entropy_workspace.argtypes = [POINTER(VocabularyLossArgs), POINTER(c_uint64)]
+        lib.snb_vocabulary_cross_entropy_workspace.restype = c_int
+        lib.snb_vocabulary_cross_entropy.argtypes = [c_void_p, POINTER(VocabularyLossArgs)]
+        lib.snb_vocabulary_cross_entropy.restype = c_int
         lib.snb_split_heads.argtypes = [c_void_p, c_void_p, c_uint64, c_void_p, c_uint64, POINTER(HeadLayout)]
         lib.snb_split_heads.restype = c_int
         lib.snb_merge_heads.argtypes = [c_void_p, c_void_p, c_uint64, c_void_p, c_uint64, POINTER(HeadLayout)]

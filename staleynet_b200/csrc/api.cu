@@ -530,6 +530,84 @@ int snb_codebook_cross_entropy(void* stream, const void* logits, int32_t logits_
     return SNB_OK;
 }
 
+namespace {
+
+// Checks of a vocabulary loss call that need no workspace.
+int check_vocabulary_loss(const snb_vocabulary_loss_args* a) {
+    if (a == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: args is null");
+    auto refuse = [](const char* what) {
+        return fail(SNB_ERR_INVALID_ARGUMENT, std::string("vocabulary_cross_entropy: ") + what);
+    };
+    const uint64_t lim = (1ull << 31) - 512;
+    auto type_ok = [](int32_t t) { return t == SNB_TYPE_F32 || t == SNB_TYPE_BF16; };
+    if (a->width == 0 || a->classes == 0) return refuse("width and classes must be at least 1");
+    // Three times the width is the longest sum (f32 operands split in two).
+    if (a->rows > lim || a->classes > lim || a->width > lim / 4) return refuse("sizes out of range");
+    if (!type_ok(a->type) || !type_ok(a->hidden_grad_type) || !type_ok(a->weight_grad_type))
+        return refuse("unknown element type");
+    if (a->type == SNB_TYPE_F32 && ((a->hidden_grad != nullptr && a->hidden_grad_type != SNB_TYPE_F32) ||
+                                    (a->weight_grad != nullptr && a->weight_grad_type != SNB_TYPE_F32)))
+        return refuse("f32 operands have f32 gradients");
+    if ((a->flags & ~SNB_GEMM_DETERMINISTIC) != 0) return refuse("unknown flags");
+    const uint64_t weight_rows = a->weight_transposed ? a->classes : a->width;
+    const uint64_t weight_cols = a->weight_transposed ? a->width : a->classes;
+    if (a->hidden_stride < a->width) return refuse("hidden_stride below the width");
+    if (a->weight_stride < weight_cols) return refuse("weight_stride below the weight's row");
+    if (a->hidden_stride > (1ull << 32) || a->weight_stride > (1ull << 32)) return refuse("stride out of range");
+    if (a->accumulate != 0 && a->weight_grad != nullptr && a->weight_grad_type == SNB_TYPE_BF16)
+        return fail(SNB_ERR_UNSUPPORTED, "vocabulary_cross_entropy: accumulating into a bf16 gradient is not supported");
+    if (a->rows > 0 && a->hidden_len < (a->rows - 1) * a->hidden_stride + a->width)
+        return fail(SNB_ERR_LEFT_TOO_SMALL, "vocabulary_cross_entropy: hidden too small");
+    if (a->weight_len < (weight_rows - 1) * a->weight_stride + weight_cols)
+        return fail(SNB_ERR_RIGHT_TOO_SMALL, "vocabulary_cross_entropy: weight too small");
+    if (a->targets_len < a->rows) return refuse("too few targets");
+    if (a->losses_len < a->rows) return fail(SNB_ERR_OUTPUT_TOO_SMALL, "vocabulary_cross_entropy: losses too small");
+    if (a->hidden_grad != nullptr && a->hidden_grad_len < a->rows * a->width)
+        return fail(SNB_ERR_OUTPUT_TOO_SMALL, "vocabulary_cross_entropy: hidden_grad too small");
+    if (a->weight_grad != nullptr && a->weight_grad_len < a->classes * a->width)
+        return fail(SNB_ERR_OUTPUT_TOO_SMALL, "vocabulary_cross_entropy: weight_grad too small");
+    if (a->weight == nullptr || (a->rows > 0 && (a->hidden == nullptr || a->targets == nullptr || a->losses == nullptr)))
+        return refuse("null pointer");
+    const uint64_t es = a->type == SNB_TYPE_BF16 ? 2 : 4;
+    auto aligned = [](const void* p, uint64_t n) { return reinterpret_cast<uintptr_t>(p) % n == 0; };
+    if (!aligned(a->hidden, es) || !aligned(a->weight, es) || !aligned(a->targets, 4) || !aligned(a->losses, 4) ||
+        !aligned(a->loss_sum, 4) || !aligned(a->hidden_grad, a->hidden_grad_type == SNB_TYPE_BF16 ? 2 : 4) ||
+        !aligned(a->weight_grad, a->weight_grad_type == SNB_TYPE_BF16 ? 2 : 4))
+        return refuse("a pointer is not aligned to its element");
+    return SNB_OK;
+}
+
+}  // namespace
+
+int snb_vocabulary_cross_entropy_workspace(const snb_vocabulary_loss_args* args, uint64_t* bytes) {
+    int rc = check_vocabulary_loss(args);
+    if (rc != SNB_OK) return rc;
+    if (bytes == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: null pointer");
+    std::string err;
+    rc = vocab_loss_workspace(*args, bytes, &err);
+    return rc == SNB_OK ? rc : fail(rc, err);
+}
+
+int snb_vocabulary_cross_entropy(void* stream, const snb_vocabulary_loss_args* args) {
+    t_last_path = SNB_PATH_NONE;
+    int rc = check_vocabulary_loss(args);
+    if (rc != SNB_OK) return rc;
+    std::string err;
+    uint64_t need = 0;
+    rc = vocab_loss_workspace(*args, &need, &err);
+    if (rc != SNB_OK) return fail(rc, err);
+    if (args->workspace_len < need || (need > 0 && args->workspace == nullptr))
+        return fail(SNB_ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: workspace holds " +
+                                                  std::to_string(args->workspace_len) + " bytes, needs " +
+                                                  std::to_string(need));
+    rc = vocab_loss_launch(static_cast<cudaStream_t>(stream), *args,
+                           t_deterministic || (args->flags & SNB_GEMM_DETERMINISTIC) != 0, t_sm_budget, &err);
+    if (rc != SNB_OK) return fail(rc, err);
+    t_last_path = args->rows == 0 ? SNB_PATH_EMPTY
+                                  : (args->rows > 128 ? SNB_PATH_TENSOR_CORE_PAIR : SNB_PATH_TENSOR_CORE);
+    return SNB_OK;
+}
+
 int snb_rms_norm_forward(void* stream, const float* input, uint64_t rows, uint64_t cols, const float* gain,
                          uint64_t gain_len, float* output, float* inv_rms, uint64_t inv_rms_len, float epsilon) {
     t_last_path = SNB_PATH_NONE;

@@ -81,13 +81,24 @@ struct TcParams {
     // side by side (tm_c 5-D: head_dim, capacity, heads, batch, P), columns (p * heads + h) * head_dim + d.
     int32_t a_heads, a_hd, a_time, a_toff;
     int32_t c_heads, c_hd, c_nheads, c_time, c_toff;
+    // Vocabulary loss epilogues (TC_EPI_LSE, TC_EPI_SOFTMAX_GRAD): the product's columns are the classes
+    // class_begin .. class_begin + N of a larger vocabulary.
+    const uint32_t* targets;  // [M] class of each row; kNoTarget: the row has none
+    int64_t class_begin;
+    float2* partials;         // LSE: [2 * tiles along N, M] (maximum, sum of 2^(log2 e x - log2 e maximum))
+    float* target_logit;      // LSE: [M], written by whoever computes the row's target column
+    const float2* row_stats;  // SOFTMAX_GRAD: [M] (log2 e maximum, log2 sum); a maximum of +inf: no gradient
 };
+
+constexpr uint32_t kNoTarget = 0xFFFFFFFFu;  // EMPTY_TOKEN (crates/staleynet-cuda/src/kernels/mod.rs:46)
 
 // Epilogue staging modes (see epilogue_tile); the host picks one per launch.
 constexpr int TC_EPI_ONE_BOX = 1;
 constexpr int TC_EPI_TWO_BOX = 2;
 constexpr int TC_EPI_AUX_BOX = 3;
-constexpr int tc_epi_boxes(int epi) { return epi == TC_EPI_ONE_BOX ? 1 : 2; }
+constexpr int TC_EPI_LSE = 4;           // row statistics of the softmax, no output tile (lse_tile)
+constexpr int TC_EPI_SOFTMAX_GRAD = 5;  // softmax minus one-hot (softmax_grad_tile)
+constexpr int tc_epi_boxes(int epi) { return epi == TC_EPI_LSE ? 0 : epi == TC_EPI_ONE_BOX ? 1 : 2; }
 
 // Shared memory of one sm_100 CTA available to a kernel.
 constexpr int TC_SMEM_LIMIT = 232448;
@@ -554,6 +565,142 @@ __device__ __forceinline__ void epilogue_tile(const TcParams& p, const CUtensorM
     }
 }
 
+// The two epilogues of the vocabulary's softmax cross entropy (vocab_loss.cu), whose logits z = A B exist only as
+// accumulator tiles in TMEM. Both work in base 2: with k = log2 e, exp(z - max) = 2^(k z - k max), one fused multiply-add
+// and one ex2.approx (relative error 2^-22) for each logit.
+//
+// lse_tile: a warp reads 32 rows x BN/2 columns (the two warps of a quadrant take the tile's two halves) and keeps each
+// row's running maximum and sum in its lane's registers: when a later 32-column piece raises the maximum from m to m',
+// the sum is multiplied by 2^(m - m'). One (maximum, sum) pair for each row and half tile goes to `partials`, so the
+// halves are joined in a fixed order by a later kernel, without atomics. The exponents are always taken against the
+// rounded product k * max, so its rounding cancels and large logits cost no more accuracy than their own rounding.
+template <int BN>
+__device__ __forceinline__ void lse_tile(const TcParams& p, const TcUnit& u, int32_t row0, uint32_t t_lane, int group) {
+    constexpr float kLog2eTile = 1.4426950408889634f;
+    if (row0 >= p.M || u.n0 + group * (BN / 2) >= p.N) return;
+    const int lane = threadIdx.x & 31;
+    const int32_t row = row0 + lane;
+    const bool live = row < p.M;
+    const uint32_t target = live ? __ldg(p.targets + row) : kNoTarget;
+    // Column of the row's target within this product; out of range (no target, another piece) matches no column.
+    const int64_t t64 = static_cast<int64_t>(target) - p.class_begin;
+    const int32_t tcol = target != kNoTarget && t64 >= 0 && t64 < p.N ? static_cast<int32_t>(t64) : -1;
+    const float kInf = __int_as_float(0x7f800000);
+    float m = -kInf, m2 = -kInf, sum = 0.0f;
+#pragma unroll 1
+    for (int c = group * (BN / 2); c < (group + 1) * (BN / 2) && u.n0 + c < p.N; c += 32) {
+        const int32_t col0 = u.n0 + c;
+        uint32_t x[32];
+        tmem_load_32x32b_x32(t_lane + c, x);
+        tmem_load_wait();
+        if (p.N - col0 < 32) {
+#pragma unroll
+            for (int j = 0; j < 32; ++j)
+                if (col0 + j >= p.N) x[j] = 0xff800000u;  // -inf: no such class
+        }
+        float top[4];
+#pragma unroll
+        for (int j = 0; j < 4; ++j) top[j] = __uint_as_float(x[j]);
+#pragma unroll
+        for (int j = 4; j < 32; ++j) top[j & 3] = fmaxf(top[j & 3], __uint_as_float(x[j]));
+        m = fmaxf(m, fmaxf(fmaxf(top[0], top[1]), fmaxf(top[2], top[3])));
+        const float top2 = __fmul_rn(m, kLog2eTile);
+        const float base = m == -kInf ? 0.0f : top2;  // every logit so far is -inf: exponents stay -inf
+        float part[4] = {sum * exp2_ftz(m2 - base), 0.0f, 0.0f, 0.0f};
+#pragma unroll
+        for (int j = 0; j < 32; ++j) part[j & 3] += exp2_ftz(fmaf(__uint_as_float(x[j]), kLog2eTile, -base));
+        sum = (part[0] + part[1]) + (part[2] + part[3]);
+        m2 = top2;
+        const int32_t local = tcol - col0;
+        if (__any_sync(0xffffffffu, local >= 0 && local < 32)) {
+            float z = 0.0f;
+#pragma unroll
+            for (int j = 0; j < 32; ++j) z = local == j ? __uint_as_float(x[j]) : z;
+            if (local >= 0 && local < 32) p.target_logit[row] = z;
+        }
+    }
+    if (live) {
+        const int64_t half = 2 * (u.n0 / BN) + group;
+        p.partials[half * p.M + row] = make_float2(m, sum);
+    }
+}
+
+// softmax_grad_tile: the same logits once more, as softmax(z) - onehot(target) with the row's statistics known. The
+// loss's scale is left to the products that read the result, so the values lie in [-1, 1] whatever the batch, and a
+// bf16 result (one rounding, relative 2^-8 at most, for the tensor cores that take it next) does not also round the scale.
+// f32 results leave as two f32 tensors for TF32 products of f32 accuracy: the 11 leading significant bits through
+// tm_c, and what they leave out through tm_lo.
+template <bool OUT_BF16, int BN>
+__device__ __forceinline__ void softmax_grad_tile(const TcParams& p, const CUtensorMap* tm_c, const CUtensorMap* tm_lo,
+                                                  const TcUnit& u, int32_t row0, uint32_t t_lane, int group,
+                                                  uint8_t* boxes, int& ebox) {
+    constexpr float kLog2eTile = 1.4426950408889634f;
+    constexpr int CHUNK = OUT_BF16 ? 64 : 32;
+    if (row0 >= p.M) return;
+    const int lane = threadIdx.x & 31;
+    const int32_t row = row0 + lane;
+    const bool live = row < p.M;
+    const uint32_t target = live ? __ldg(p.targets + row) : kNoTarget;
+    // 2^(k z - k max - log2 sum) in two steps: their sum in one f32 would round by up to 2^-24 of itself, a relative
+    // error of that size times ln 2 in every value of the row.
+    const float2 stats = live ? __ldg(p.row_stats + row) : make_float2(0.0f, 0.0f);
+    const float2 base = f2(-stats.x), rest = f2(-stats.y);
+    const int64_t t64 = static_cast<int64_t>(target) - p.class_begin;
+    const int32_t tcol = target != kNoTarget && t64 >= 0 && t64 < p.N ? static_cast<int32_t>(t64) : -1;
+#pragma unroll 1
+    for (int c = group * CHUNK; c < BN && u.n0 + c < p.N; c += 2 * CHUNK) {
+        const int32_t col0 = u.n0 + c;
+        uint8_t* box = boxes + (OUT_BF16 ? ebox * TC_EPI_BOX_BYTES : 0);
+        if (lane == 0) {
+            if constexpr (OUT_BF16) bulk_wait_group_read<1>();  // only the store before last used this box
+            else bulk_wait_group_read<0>();                     // both boxes are rewritten
+        }
+        __syncwarp();
+#pragma unroll
+        for (int h = 0; h < CHUNK / 32; ++h) {
+            uint32_t x[32];
+            tmem_load_32x32b_x32(t_lane + c + 32 * h, x);
+            tmem_load_wait();
+            float2 v[16];
+#pragma unroll
+            for (int j = 0; j < 16; ++j) {
+                const float2 z = make_float2(__uint_as_float(x[2 * j]), __uint_as_float(x[2 * j + 1]));
+                const float2 e = __fadd2_rn(__ffma2_rn(z, f2(kLog2eTile), base), rest);
+                v[j] = make_float2(exp2_ftz(e.x), exp2_ftz(e.y));
+            }
+            const int32_t local = tcol - (col0 + 32 * h);
+            if (__any_sync(0xffffffffu, local >= 0 && local < 32)) {
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    v[j].x -= local == 2 * j ? 1.0f : 0.0f;
+                    v[j].y -= local == 2 * j + 1 ? 1.0f : 0.0f;
+                }
+            }
+            if constexpr (!OUT_BF16) {
+                float2 low[16];
+#pragma unroll
+                for (int j = 0; j < 16; ++j) {
+                    const float2 full = v[j];
+                    // The nearest value of 11 significant bits (|full| <= 1, so the carry stays in range).
+                    v[j].x = __uint_as_float((__float_as_uint(full.x) + 0x1000u) & 0xffffe000u);
+                    v[j].y = __uint_as_float((__float_as_uint(full.y) + 0x1000u) & 0xffffe000u);
+                    low[j] = make_float2(full.x - v[j].x, full.y - v[j].y);
+                }
+                stage_half<OUT_BF16>(boxes + TC_EPI_BOX_BYTES, lane, h, low);
+            }
+            stage_half<OUT_BF16>(box, lane, h, v);
+        }
+        fence_proxy_async_shared();
+        __syncwarp();
+        if (lane == 0) {
+            tma_store_3d(tm_c, smem_addr(box), col0, row0, 0);
+            if constexpr (!OUT_BF16) tma_store_3d(tm_lo, smem_addr(boxes + TC_EPI_BOX_BYTES), col0, row0, 0);
+            bulk_commit_group();
+        }
+        if constexpr (OUT_BF16) ebox ^= 1;
+    }
+}
+
 // The bias feed of SB kernels: the producer copies tile t's BN bias values into buffer t & 1 of `bias_s` once the
 // epilogue warps have released that buffer from tile t - 2 (bias_empty), completion on bias_full[t & 1].
 template <int BN>
@@ -775,8 +922,13 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
             const int32_t row0 = u.m0 + q * 32;
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
 
-            epilogue_tile<OUT_BF16, BN, EPI, SB>(p, &tm_c, &tm_pre, u, row0, t_lane, group, boxes, ebox, aux_bar,
-                                                 aux_phase, bias_s + static_cast<uint32_t>(acc * BN * 4));
+            if constexpr (EPI == TC_EPI_LSE)
+                lse_tile<BN>(p, u, row0, t_lane, group);
+            else if constexpr (EPI == TC_EPI_SOFTMAX_GRAD)
+                softmax_grad_tile<OUT_BF16, BN>(p, &tm_c, &tm_pre, u, row0, t_lane, group, boxes, ebox);
+            else
+                epilogue_tile<OUT_BF16, BN, EPI, SB>(p, &tm_c, &tm_pre, u, row0, t_lane, group, boxes, ebox, aux_bar,
+                                                     aux_phase, bias_s + static_cast<uint32_t>(acc * BN * 4));
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) {

@@ -247,8 +247,13 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
             const int32_t row0 = u.m0 + row_off;
             const uint32_t t_lane = tmem_base + (static_cast<uint32_t>(q * 32) << 16) + acc * BN;
 
-            epilogue_tile<OUT_BF16, BN, EPI, SB>(p, &tm_c, &tm_pre, u, row0, t_lane, group, boxes, ebox, aux_bar,
-                                                 aux_phase, bias_s + static_cast<uint32_t>(acc * BN * 4));
+            if constexpr (EPI == TC_EPI_LSE)
+                lse_tile<BN>(p, u, row0, t_lane, group);
+            else if constexpr (EPI == TC_EPI_SOFTMAX_GRAD)
+                softmax_grad_tile<OUT_BF16, BN>(p, &tm_c, &tm_pre, u, row0, t_lane, group, boxes, ebox);
+            else
+                epilogue_tile<OUT_BF16, BN, EPI, SB>(p, &tm_c, &tm_pre, u, row0, t_lane, group, boxes, ebox, aux_bar,
+                                                     aux_phase, bias_s + static_cast<uint32_t>(acc * BN * 4));
             tcgen05_fence_before_sync();
             __syncwarp();
             if (lane == 0) {

@@ -31,6 +31,7 @@ struct GemmRequest {
     const snb_head_layout* a_heads;  // left operand read from its head-major form, or nullptr (snb_gemm_args)
     const snb_head_layout* c_heads;  // output written head-major, or nullptr
     int sm_budget;            // SMs the persistent grid may occupy (0: all; snb_set_sm_budget)
+    uint64_t max_split_inner; // longest sum of one split of K where K may be split (0: as the cost model has it)
 };
 
 struct DeviceInfo {
@@ -104,6 +105,36 @@ int bounded_wait_probe(cudaStream_t stream, uint64_t limit_ns, std::string* err)
 
 // Reads and clears the tensor-core kernels' device status word on the current device (synchronizes first).
 int read_and_clear_device_status(unsigned int* status, std::string* err);
+
+// One product of the vocabulary's softmax cross entropy (tc_gemm.cu): logits = A B for `classes` classes from
+// class_begin on, A [rows, inner] (K-major, rows a_ld elements apart), B [classes, inner] (rows b_ld apart) or with
+// b_mn_major [inner, classes]; bf16, or f32 on TF32 tensor cores. Without `grad` the row statistics are written
+// (partials, target_logit); with it softmax minus one-hot, as bf16 [rows, grad_ld], or for f32 operands as the two
+// f32 tensors grad and grad_low whose sum it is. Bases and row pitches are multiples of 16 bytes.
+struct VocabProduct {
+    int type;
+    uint64_t rows, classes, inner;
+    const void* A;
+    uint64_t a_ld;
+    const void* B;
+    uint64_t b_ld;
+    bool b_mn_major;
+    const uint32_t* targets;
+    int64_t class_begin;
+    float2* partials;
+    float* target_logit;
+    const float2* row_stats;
+    void* grad;
+    void* grad_low;
+    uint64_t grad_ld;
+    int sm_budget;
+};
+int tc_vocab_product(cudaStream_t stream, const VocabProduct& v, std::string* err);
+
+// Softmax cross entropy over a vocabulary in pieces (vocab_loss.cu).
+int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std::string* err);
+int vocab_loss_launch(cudaStream_t stream, const snb_vocabulary_loss_args& a, bool deterministic, int sm_budget,
+                      std::string* err);
 
 std::string cuda_message(const char* what, cudaError_t e);
 

@@ -376,7 +376,9 @@ int tc_gemm_try(cudaStream_t stream, const GemmRequest& r, bool* launched, int* 
                            ? choose_splits(tiles, k_blocks, workers, slice_flops, pair ? 2.0 * sm_flops : sm_flops,
                                            slab_mode ? 2.0 * out_bytes : out_bytes, slab_mode || p.accumulate == 0)
                            : 1;
-    const int64_t kb_per_split = (k_blocks + splits - 1) / splits;
+    int64_t kb_per_split = (k_blocks + splits - 1) / splits;
+    if (r.max_split_inner > 0 && plain_epilogue && !r.deterministic)
+        kb_per_split = std::min(kb_per_split, std::max<int64_t>(1, static_cast<int64_t>(r.max_split_inner) / bk));
     const int64_t splits_used = (k_blocks + kb_per_split - 1) / kb_per_split;  // every split has >= 1 slice
     const bool slabs = slab_mode && splits_used > 1;
 
@@ -620,6 +622,87 @@ int tc_gemm_try(cudaStream_t stream, const GemmRequest& r, bool* launched, int* 
     if (rc == SNB_OK) rc = sum_slabs();
     if (rc == SNB_OK) *launched = true;
     return rc;
+}
+
+int tc_vocab_product(cudaStream_t stream, const VocabProduct& v, std::string* err) {
+    DeviceInfo dev;
+    int rc = current_device_info(&dev, err);
+    if (rc != SNB_OK) return rc;
+    if (dev.major != 10) {
+        *err = "vocabulary cross entropy needs an sm_100 device";
+        return SNB_ERR_UNSUPPORTED;
+    }
+    const bool bf16 = v.type == SNB_TYPE_BF16;
+    const int esize = bf16 ? 2 : 4;
+    const uint32_t bk = 128 / esize, mn_box = 128 / esize;
+    const int sms = v.sm_budget > 0 ? std::min(v.sm_budget, dev.sm_count) : dev.sm_count;
+    // CTA pairs whenever a pair's second CTA has rows of its own (see tc_gemm_try for what pairs save).
+    const bool pair = v.rows > TC_BM && sms >= 2;
+    const int64_t bm = pair ? TC2_BM : TC_BM, bn = 256;
+    const int64_t m_tiles = (static_cast<int64_t>(v.rows) + bm - 1) / bm;
+    const int64_t n_tiles = (static_cast<int64_t>(v.classes) + bn - 1) / bn;
+    if (m_tiles * n_tiles > (1ll << 30)) {
+        *err = "vocabulary cross entropy: too many tiles";
+        return SNB_ERR_UNSUPPORTED;
+    }
+    CUtensorMap maps[7];
+    const CUtensorMapDataType in_dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_TFLOAT32;
+    if (!encode_3d(&maps[0], in_dt, esize, v.A, v.inner, v.rows, 1, v.a_ld, v.a_ld * v.rows, bk, TC_BM, err))
+        return SNB_ERR_CUDA;
+    if (v.b_mn_major) {
+        if (!encode_3d(&maps[1], in_dt, esize, v.B, v.classes, v.inner, 1, v.b_ld, v.b_ld * v.inner, mn_box, bk, err,
+                       bf16 ? CU_TENSOR_MAP_SWIZZLE_128B : CU_TENSOR_MAP_SWIZZLE_128B_ATOM_32B))
+            return SNB_ERR_CUDA;
+    } else if (!encode_3d(&maps[1], in_dt, esize, v.B, v.inner, v.classes, 1, v.b_ld, v.b_ld * v.classes, bk,
+                          static_cast<uint32_t>(pair ? bn / 2 : bn), err)) {
+        return SNB_ERR_CUDA;
+    }
+    maps[2] = maps[3] = maps[0];  // the statistics epilogue stores no tile
+    if (v.grad != nullptr) {
+        const CUtensorMapDataType out_dt = bf16 ? CU_TENSOR_MAP_DATA_TYPE_BFLOAT16 : CU_TENSOR_MAP_DATA_TYPE_FLOAT32;
+        const uint32_t chunk = bf16 ? 64 : 32;
+        if (!encode_3d(&maps[2], out_dt, esize, v.grad, v.classes, v.rows, 1, v.grad_ld, v.grad_ld * v.rows, chunk, 32,
+                       err))
+            return SNB_ERR_CUDA;
+        if (!bf16 && !encode_3d(&maps[3], out_dt, esize, v.grad_low, v.classes, v.rows, 1, v.grad_ld,
+                                v.grad_ld * v.rows, chunk, 32, err))
+            return SNB_ERR_CUDA;
+    }
+    maps[4] = maps[5] = maps[6] = maps[2];
+
+    TcParams p{};
+    p.M = static_cast<int32_t>(v.rows);
+    p.N = static_cast<int32_t>(v.classes);
+    p.K = static_cast<int32_t>(v.inner);
+    p.count = 1;
+    p.b_mn_major = v.b_mn_major;
+    p.m_tiles = static_cast<int32_t>(m_tiles);
+    p.n_tiles = static_cast<int32_t>(n_tiles);
+    p.k_blocks = static_cast<int32_t>((v.inner + bk - 1) / bk);
+    p.splits = 1;
+    p.k_blocks_per_split = p.k_blocks;
+    p.num_units = static_cast<int32_t>(m_tiles * n_tiles);
+    p.m_fastest = v.classes > v.rows ? 1 : 0;
+    p.scale = 1.0f;
+    p.targets = v.targets;
+    p.class_begin = v.class_begin;
+    p.partials = v.partials;
+    p.target_logit = v.target_logit;
+    p.row_stats = v.row_stats;
+    const int workers = pair ? sms / 2 : sms;
+    const int grid = static_cast<int>(std::min<int64_t>(p.num_units, workers)) * (pair ? 2 : 1);
+    using B = __nv_bfloat16;
+    const CUtensorMap* m = maps;
+#define SNB_ONE(E_, OB_, EPI_) launch<E_, 256, OB_, EPI_>(stream, m[0], m[1], m[2], m[3], m[4], m[5], m[6], p, grid, err)
+#define SNB_PAIR(E_, OB_, EPI_) launch_pair<E_, OB_, EPI_>(stream, m, p, grid, err)
+    if (v.grad == nullptr) {
+        if (bf16) return pair ? SNB_PAIR(B, false, TC_EPI_LSE) : SNB_ONE(B, false, TC_EPI_LSE);
+        return pair ? SNB_PAIR(float, false, TC_EPI_LSE) : SNB_ONE(float, false, TC_EPI_LSE);
+    }
+    if (bf16) return pair ? SNB_PAIR(B, true, TC_EPI_SOFTMAX_GRAD) : SNB_ONE(B, true, TC_EPI_SOFTMAX_GRAD);
+    return pair ? SNB_PAIR(float, false, TC_EPI_SOFTMAX_GRAD) : SNB_ONE(float, false, TC_EPI_SOFTMAX_GRAD);
+#undef SNB_ONE
+#undef SNB_PAIR
 }
 
 int fused_attention_forward(cudaStream_t stream, const void* q, const void* k, const void* v, uint64_t count,

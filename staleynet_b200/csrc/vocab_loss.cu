@@ -1,0 +1,509 @@
+// vocab_loss.cu — softmax cross entropy over a large vocabulary, with its gradients, without keeping the logits.
+//
+//   z = H W^T,  lse_i = log sum_v exp(z_iv),  loss_i = lse_i - z_it,  P = softmax(z) - onehot(t)
+//   dH = c P W,  dW = c P^T H
+//
+// Pass 1 computes z tile by tile on the tensor cores and reduces each tile in its epilogue to one (maximum, sum) pair
+// for each row and 128 classes (lse_tile in gemm_tc.cuh); combine_kernel joins the pairs of a row in a fixed order. Pass
+// 2, for gradients, takes the vocabulary in pieces: each piece's tiles of z are computed again, turned into P in the
+// epilogue (softmax_grad_tile), and the piece of P is the operand of two ordinary products. No logits are kept: the
+// piece of P is bounded by kPieceBytes, and the pairs of pass 1 take one byte for each 16 logits.
+//
+// What bounds it: the products, 2 rows x width x classes operations for the loss and 8 for loss and gradients (6 and
+// the second computation of z), except for a few rows, where it is the one (loss) or three (gradients) passes over the
+// weight.
+//
+// f32 operands: x = hi + lo with hi its nearest value of 11 significant bits and lo the rest's, and
+// x y = lo hi' + hi lo' + hi hi' up to 2^-22 of |x y|: three TF32 products with f32 sums. The logits take them as one
+// product over three times the width (H packed as lo|hi|hi, W as hi|lo|hi), so that the epilogue sees whole logits; the
+// tensor core cuts off what a sum's last bit cannot hold at every instruction, so the small products come first, where
+// that costs little. The gradient products add one after the other into f32 outputs.
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "internal.h"
+
+namespace snb {
+namespace {
+
+constexpr uint32_t kEmptyToken = 0xFFFFFFFFu;      // EMPTY_TOKEN (kernels/mod.rs:46)
+constexpr uint64_t kPieceBytes = 256ull << 20;     // bound of a piece of P (and of a packed piece of the weight)
+// Longest sum of f32 products on the tensor core, which cuts off the accumulator's lost bits at each instruction (8
+// products) instead of rounding: 2^-24 of the sum each time on average, always towards zero. Measured as the relative
+// error of a weight gradient over 1,021 rows: 2.5e-6 in one sum, 0.7e-6 in sums of 256 (0.6e-6 with f32 arithmetic).
+constexpr uint64_t kSumLength = 256;
+constexpr float kLog2e = 1.4426950408889634f;
+constexpr uint64_t kHalfTile = 128;                // classes that one (maximum, sum) pair covers
+
+__device__ __forceinline__ uint16_t bf16_bits(float f) {
+    const uint32_t u = __float_as_uint(f);
+    if ((u & 0x7FFFFFFFu) > 0x7F800000u) return static_cast<uint16_t>((u >> 16) | 0x40u);  // NaN stays NaN
+    return static_cast<uint16_t>((u + 0x7FFFu + ((u >> 16) & 1u)) >> 16);
+}
+
+// A packed copy of a row-major matrix: dst[i, j] = src[i, j] (rows src_ld and dst_ld elements apart), zero outside
+// [rows, cols] up to [dst_rows, dst_cols] and in the rows that have no target (`targets`, may be null): their hidden
+// vectors may hold anything, and 0 * NaN must not reach the weight's gradient. bf16 stays bf16; f32 becomes three
+// planes of TF32 values, plane k at dst + plane[k], holding the leading part (low bit k of `low` clear) or the rest.
+struct PackParams {
+    const void* src;
+    int64_t src_ld, rows, cols;
+    void* dst;
+    int64_t dst_ld, dst_rows, dst_cols;
+    const uint32_t* targets;
+    int64_t plane[3];
+    int32_t low;
+};
+
+__global__ void __launch_bounds__(256) pack_bf16_kernel(const PackParams p) {
+    const int64_t total = p.dst_rows * p.dst_cols;
+    const uint16_t* src = static_cast<const uint16_t*>(p.src);
+    uint16_t* dst = static_cast<uint16_t*>(p.dst);
+    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
+         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t i = e / p.dst_cols, j = e - i * p.dst_cols;
+        const bool live = i < p.rows && j < p.cols && (p.targets == nullptr || __ldg(p.targets + i) != kEmptyToken);
+        dst[i * p.dst_ld + j] = live ? src[i * p.src_ld + j] : 0;
+    }
+}
+
+// The nearest value of 11 significant bits; a finite value that would round past the largest float is cut off instead.
+__device__ __forceinline__ float tf32_nearest(float x) {
+    const uint32_t u = __float_as_uint(x);
+    const uint32_t r = (u + 0x0FFFu + ((u >> 13) & 1u)) & 0xFFFFE000u;
+    return __uint_as_float((r & 0x7F800000u) == 0x7F800000u ? u & 0xFFFFE000u : r);
+}
+
+__global__ void __launch_bounds__(256) pack_split_kernel(const PackParams p) {
+    const int64_t total = p.dst_rows * p.dst_cols;
+    const float* src = static_cast<const float*>(p.src);
+    float* dst = static_cast<float*>(p.dst);
+    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
+         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t i = e / p.dst_cols, j = e - i * p.dst_cols;
+        const bool live = i < p.rows && j < p.cols && (p.targets == nullptr || __ldg(p.targets + i) != kEmptyToken);
+        const float x = live ? src[i * p.src_ld + j] : 0.0f;
+        // An infinity or NaN stays whole in the leading part (inf - inf would make the rest NaN).
+        const bool finite = (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
+        const float hi = finite ? tf32_nearest(x) : x;
+        const float lo = finite ? tf32_nearest(x - hi) : 0.0f;
+#pragma unroll
+        for (int k = 0; k < 3; ++k) dst[p.plane[k] + i * p.dst_ld + j] = (p.low >> k) & 1 ? lo : hi;
+    }
+}
+
+// out[i, j] (+)= ws[i, j] for i < rows, j < cols.
+__global__ void __launch_bounds__(256) store_kernel(const float* ws, int64_t ws_ld, void* out, int out_bf16,
+                                                    int64_t out_ld, int64_t rows, int64_t cols, int accumulate) {
+    const int64_t total = rows * cols;
+    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
+         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
+        const int64_t i = e / cols, j = e - i * cols;
+        const float v = ws[i * ws_ld + j];
+        if (out_bf16) {
+            static_cast<uint16_t*>(out)[i * out_ld + j] = bf16_bits(v);
+        } else {
+            float* o = static_cast<float*>(out) + i * out_ld + j;
+            *o = accumulate ? *o + v : v;
+        }
+    }
+}
+
+constexpr int kCombineRows = 32, kCombineLanes = 32;
+
+// Joins the (maximum, sum) pairs of each row: the block's 32 rows lie along the threads of a warp (coalesced
+// reads), its 32 warps take every 32nd pair, and their results are joined in warp order, so the result does not depend
+// on scheduling. Writes the row's loss and, for pass 2, (log2 e maximum, log2 sum), with a maximum of +inf in a row
+// without a target (every exponential is then 0) and NaN for a target that is no class. A grid of one block
+// also writes the sum of the losses.
+__global__ void __launch_bounds__(kCombineRows * kCombineLanes)
+    combine_kernel(const float2* partials, int64_t pairs, int64_t rows, const uint32_t* targets, uint64_t classes,
+                   const float* target_logit, float* losses, float2* row_stats, float* loss_sum) {
+    __shared__ float2 part[kCombineLanes][kCombineRows];
+    const int r = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
+    const float inf = __int_as_float(0x7f800000);
+    float m = -inf, s = 0.0f;
+    auto join = [&](float2 v) {
+        const float next = fmaxf(m, v.x);
+        const float base = next == -inf ? 0.0f : __fmul_rn(next, kLog2e);
+        s = s * exp2f(__fmul_rn(m, kLog2e) - base) + v.y * exp2f(__fmul_rn(v.x, kLog2e) - base);
+        m = next;
+    };
+    if (row < rows) {
+#pragma unroll 4
+        for (int64_t k = w; k < pairs; k += kCombineLanes) join(__ldg(partials + k * rows + row));
+    }
+    part[w][r] = make_float2(m, s);
+    __syncthreads();
+    if (w != 0) return;
+    m = -inf;
+    s = 0.0f;
+    for (int k = 0; k < kCombineLanes; ++k) join(part[k][r]);
+    float loss = 0.0f;
+    if (row < rows) {
+        const uint32_t t = targets[row];
+        const float nan = __int_as_float(0x7fc00000);
+        if (t != kEmptyToken) loss = t < classes ? (m - target_logit[row]) + logf(s) : nan;
+        losses[row] = loss;
+        if (row_stats != nullptr)
+            row_stats[row] = t == kEmptyToken ? make_float2(inf, 0.0f)
+                                              : make_float2(t < classes ? __fmul_rn(m, kLog2e) : nan, log2f(s));
+    }
+    if (loss_sum != nullptr && gridDim.x == 1) {
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, d);
+        if (r == 0) *loss_sum = loss;
+    }
+}
+
+// The sum of the losses of more than 32 rows: one block, each thread every 1024th row, then a tree.
+__global__ void __launch_bounds__(1024) loss_sum_kernel(const float* losses, int64_t rows, float* loss_sum) {
+    __shared__ double part[32];
+    double s = 0.0;
+    for (int64_t i = threadIdx.x; i < rows; i += 1024) s += static_cast<double>(losses[i]);
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = s;
+    __syncthreads();
+    if (threadIdx.x < 32) {
+        s = part[threadIdx.x];
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1) s += __shfl_xor_sync(0xffffffffu, s, d);
+        if (threadIdx.x == 0) *loss_sum = static_cast<float>(s);
+    }
+}
+
+uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
+
+// The shapes and the workspace of one call. Offsets are from a 256-byte aligned base.
+struct Layout {
+    bool f32, gradients, pack_hidden, pack_weight;
+    uint64_t elem;          // bytes of an operand element
+    uint64_t seg;           // width rounded up to 16 bytes: a packed row, or one of the three planes of an f32 row
+    uint64_t k_logits;      // length of the logits' sums
+    uint64_t piece, pieces; // classes of a piece (the last one may have fewer) and pieces
+    uint64_t hidden_ld, weight_ld;   // of the operands that the products read
+    uint64_t grad_ld;       // of a piece of P
+    uint64_t wgrad_ld, wgrad_rows;   // f32 weight gradient of a piece before it is stored
+    uint64_t hidden_at, weight_at, partials_at, target_at, stats_at, p_at, dh_at, dw_at, bytes;
+};
+
+bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
+
+Layout layout_of(const snb_vocabulary_loss_args& a) {
+    Layout l{};
+    l.f32 = a.type == SNB_TYPE_F32;
+    l.gradients = a.hidden_grad != nullptr || a.weight_grad != nullptr;
+    l.elem = l.f32 ? 4 : 2;
+    const uint64_t per16 = 16 / l.elem;
+    l.seg = round_up(a.width, per16);
+    l.k_logits = l.f32 ? 3 * l.seg : a.width;
+    // The weight's gradient multiplies by the hidden rows without a target too: those have to be zero then.
+    l.pack_hidden = l.f32 || a.weight_grad != nullptr || !aligned16(a.hidden) || a.hidden_stride % per16 != 0;
+    // (The hidden gradient's product has `seg` columns: those past the width must be zeros of a packed weight.)
+    l.pack_weight = l.f32 || !aligned16(a.weight) || a.weight_stride % per16 != 0 ||
+                    (a.hidden_grad != nullptr && a.width != l.seg);
+    // A piece is as long as the bound allows for P [rows, piece] and for the packed weight, in whole tiles.
+    uint64_t piece = round_up(a.classes, 256);
+    auto bound = [&](uint64_t bytes_a_class) {
+        piece = std::min(piece, std::max<uint64_t>(256, kPieceBytes / std::max<uint64_t>(1, bytes_a_class) / 256 * 256));
+    };
+    if (l.gradients) bound(a.rows * (l.f32 ? 8 : 2));
+    if (l.pack_weight) bound(l.f32 ? 12 * l.seg : 2 * l.seg);
+    l.piece = std::min(piece, a.classes);
+    l.pieces = (a.classes + l.piece - 1) / l.piece;
+    const uint64_t piece_ld = round_up(l.piece, 8);
+    l.hidden_ld = l.pack_hidden ? (l.f32 ? 3 * l.seg : l.seg) : a.hidden_stride;
+    l.weight_ld = !l.pack_weight ? a.weight_stride
+                                 : a.weight_transposed ? (l.f32 ? 3 * l.seg : l.seg) : piece_ld;
+    l.grad_ld = piece_ld;
+    l.wgrad_rows = a.weight_transposed ? l.piece : l.seg;
+    l.wgrad_ld = a.weight_transposed ? l.seg : piece_ld;
+    uint64_t at = 0;
+    auto take = [&](uint64_t bytes) {
+        const uint64_t here = at;
+        at += round_up(bytes, 256);
+        return here;
+    };
+    l.hidden_at = take(l.pack_hidden ? a.rows * l.hidden_ld * l.elem : 0);
+    l.weight_at = take(l.pack_weight ? (a.weight_transposed ? l.piece * l.weight_ld
+                                                            : (l.f32 ? 3 : 1) * l.seg * l.weight_ld) * l.elem : 0);
+    l.partials_at = take((a.classes + kHalfTile - 1) / kHalfTile * a.rows * sizeof(float2));
+    l.target_at = take(a.rows * 4);
+    l.stats_at = take(a.rows * sizeof(float2));
+    l.p_at = take(l.gradients ? a.rows * l.grad_ld * (l.f32 ? 8 : 2) : 0);
+    l.dh_at = take(a.hidden_grad != nullptr ? a.rows * l.seg * 4 : 0);
+    l.dw_at = take(a.weight_grad != nullptr ? l.wgrad_rows * l.wgrad_ld * 4 : 0);
+    l.bytes = a.rows == 0 ? 0 : at + 256;
+    return l;
+}
+
+int launched(const char* what, std::string* err) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return SNB_OK;
+    *err = cuda_message(what, e);
+    return SNB_ERR_CUDA;
+}
+
+unsigned flat_grid(uint64_t elements, int sms) {
+    return static_cast<unsigned>(std::max<uint64_t>(1, std::min<uint64_t>((elements + 255) / 256, 8ull * sms)));
+}
+
+// One call's stream, arguments and choices, and the products it issues.
+struct Call {
+    cudaStream_t stream;
+    const snb_vocabulary_loss_args& a;
+    const Layout l;
+    bool deterministic;
+    int sm_budget, sms;
+    uint8_t* base;
+    std::string* err;
+
+    void* at(uint64_t offset) const { return base + offset; }
+
+    // An operand of a gradient product; for f32 its leading parts, with the rest at `low` in the same layout.
+    struct Part {
+        const void* lead;
+        const void* low;
+    };
+
+    int pack(const void* src, uint64_t src_ld, uint64_t rows, uint64_t cols, void* dst, uint64_t dst_ld,
+             uint64_t dst_rows, uint64_t dst_cols, const uint32_t* targets, uint64_t plane, int low) const {
+        PackParams p{};
+        p.src = src;
+        p.src_ld = static_cast<int64_t>(src_ld);
+        p.rows = static_cast<int64_t>(rows);
+        p.cols = static_cast<int64_t>(cols);
+        p.dst = dst;
+        p.dst_ld = static_cast<int64_t>(dst_ld);
+        p.dst_rows = static_cast<int64_t>(dst_rows);
+        p.dst_cols = static_cast<int64_t>(dst_cols);
+        p.targets = targets;
+        for (int k = 0; k < 3; ++k) p.plane[k] = static_cast<int64_t>(k * plane);
+        p.low = low;
+        const unsigned grid = flat_grid(dst_rows * dst_cols, sms);
+        if (l.f32) pack_split_kernel<<<grid, 256, 0, stream>>>(p);
+        else pack_bf16_kernel<<<grid, 256, 0, stream>>>(p);
+        return launched("vocabulary loss pack kernel launch", err);
+    }
+
+    const void* hidden() const { return l.pack_hidden ? at(l.hidden_at) : a.hidden; }
+
+    Part hidden_part() const {
+        const float* h = static_cast<const float*>(at(l.hidden_at));
+        return l.f32 ? Part{h + l.seg, h} : Part{hidden(), nullptr};
+    }
+
+    Part weight_part(const void* w) const {
+        const uint64_t plane = a.weight_transposed ? l.seg : l.seg * l.weight_ld;
+        return l.f32 ? Part{w, static_cast<const float*>(w) + plane} : Part{w, nullptr};
+    }
+
+    Part grad_part() const {
+        const void* p = at(l.p_at);
+        return l.f32 ? Part{p, static_cast<const float*>(p) + a.rows * l.grad_ld} : Part{p, nullptr};
+    }
+
+    // The weight of the classes from v0 on, packed into the workspace where the products cannot read it in place.
+    int weight(uint64_t v0, uint64_t n, const void** w) const {
+        const uint64_t offset = (a.weight_transposed ? v0 * a.weight_stride : v0) * l.elem;
+        const void* src = static_cast<const uint8_t*>(a.weight) + offset;
+        *w = src;
+        if (!l.pack_weight) return SNB_OK;
+        *w = at(l.weight_at);
+        constexpr int kHiLoHi = 2;
+        if (a.weight_transposed)
+            return pack(src, a.weight_stride, n, a.width, at(l.weight_at), l.weight_ld, n, l.seg, nullptr, l.seg, kHiLoHi);
+        return pack(src, a.weight_stride, a.width, n, at(l.weight_at), l.weight_ld, l.seg, round_up(n, 8), nullptr,
+                    l.seg * l.weight_ld, kHiLoHi);
+    }
+
+    VocabProduct logits(uint64_t v0, uint64_t n, const void* w) const {
+        VocabProduct v{};
+        v.type = a.type;
+        v.rows = a.rows;
+        v.classes = n;
+        v.inner = l.k_logits;
+        v.A = hidden();
+        v.a_ld = l.hidden_ld;
+        v.B = w;
+        v.b_ld = l.weight_ld;
+        v.b_mn_major = a.weight_transposed == 0;
+        v.targets = a.targets;
+        v.class_begin = static_cast<int64_t>(v0);
+        v.partials = static_cast<float2*>(at(l.partials_at)) + v0 / kHalfTile * a.rows;
+        v.target_logit = static_cast<float*>(at(l.target_at));
+        v.row_stats = static_cast<const float2*>(at(l.stats_at));
+        v.sm_budget = sm_budget;
+        return v;
+    }
+
+    // C [rows, cols] (dense) (+)= grad_scale * A B; for f32 the three products of the split operands.
+    int product(uint64_t rows, uint64_t cols, uint64_t inner, Part A, snb_operand left, Part B, snb_operand right,
+                void* C, int c_type, bool accumulate) const {
+        GemmRequest r{};
+        r.p.rows = rows;
+        r.p.cols = cols;
+        r.p.inner = inner;
+        r.p.left = left;
+        r.p.right = right;
+        r.p.scale = a.grad_scale;
+        r.p.accumulate = accumulate ? 1 : 0;
+        r.count = 1;
+        r.a_type = r.b_type = a.type;
+        r.c_type = c_type;
+        r.precision = l.f32 ? SNB_PRECISION_TF32 : SNB_PRECISION_BF16;
+        r.C = C;
+        r.aux_type = c_type;
+        r.deterministic = deterministic;
+        r.sm_budget = sm_budget;
+        auto issue = [&]() {
+            bool tensor = false;
+            int path = 0;
+            int rc = tc_gemm_try(stream, r, &tensor, &path, err);
+            if (rc == SNB_OK && !tensor) rc = simt_gemm(stream, r, err);
+            r.p.accumulate = 1;
+            return rc;
+        };
+        r.A = l.f32 ? A.low : A.lead;
+        r.B = B.lead;
+        int rc = issue();
+        if (rc != SNB_OK || !l.f32) return rc;
+        r.A = A.lead;
+        r.B = B.low;
+        if ((rc = issue()) != SNB_OK) return rc;
+        // The leading parts' product in sums of kSumLength, which meet in f32 additions that round to nearest: as splits
+        // of one launch, or in the deterministic mode as one launch after the other.
+        r.B = B.lead;
+        if (!deterministic) {
+            r.max_split_inner = kSumLength;
+            return issue();
+        }
+        for (uint64_t k = 0; k < inner && rc == SNB_OK; k += kSumLength) {
+            r.p.inner = std::min(kSumLength, inner - k);
+            r.A = static_cast<const float*>(A.lead) + k * left.col_stride;
+            r.B = static_cast<const float*>(B.lead) + k * right.row_stride;
+            rc = issue();
+        }
+        return rc;
+    }
+
+    int store(const void* ws, uint64_t ws_ld, void* out, int out_type, uint64_t out_ld, uint64_t rows, uint64_t cols,
+              bool accumulate) const {
+        store_kernel<<<flat_grid(rows * cols, sms), 256, 0, stream>>>(
+            static_cast<const float*>(ws), static_cast<int64_t>(ws_ld), out, out_type == SNB_TYPE_BF16,
+            static_cast<int64_t>(out_ld), static_cast<int64_t>(rows), static_cast<int64_t>(cols), accumulate);
+        return launched("vocabulary loss store kernel launch", err);
+    }
+
+    // dH (+)= P W of one piece, into the f32 sums.
+    int hidden_grad(uint64_t v0, uint64_t n, const void* w) const {
+        const snb_operand left{l.grad_ld, 1, 0};
+        const snb_operand right = a.weight_transposed ? snb_operand{l.weight_ld, 1, 0} : snb_operand{1, l.weight_ld, 0};
+        return product(a.rows, l.seg, n, grad_part(), left, weight_part(w), right, at(l.dh_at), SNB_TYPE_F32, v0 > 0);
+    }
+
+    // dW (+)= P^T H of one piece (or its transpose, for a [width, classes] weight).
+    int weight_grad(uint64_t v0, uint64_t n) const {
+        const uint64_t es = a.weight_grad_type == SNB_TYPE_BF16 ? 2 : 4;
+        const snb_operand p_t{1, l.grad_ld, 0}, h{l.hidden_ld, 1, 0}, h_t{1, l.hidden_ld, 0}, p_n{l.grad_ld, 1, 0};
+        uint8_t* out = static_cast<uint8_t*>(a.weight_grad) + (a.weight_transposed ? v0 * a.width : v0) * es;
+        int rc;
+        if (a.weight_transposed) {
+            // The rows of the piece are contiguous in the gradient: written there unless a row is no multiple of 16
+            // bytes, or a bf16 gradient has so few tiles that its sums are better split (which needs f32).
+            const bool dense = a.width * es % 16 == 0 && aligned16(out);
+            const uint64_t tiles = (n + 255) / 256 * ((a.width + 255) / 256), pairs = static_cast<uint64_t>(sms / 2);
+            const bool fills = tiles * 10 >= (tiles + pairs - 1) / pairs * pairs * 6;
+            if (dense && (a.weight_grad_type == SNB_TYPE_F32 || fills))
+                return product(n, a.width, a.rows, grad_part(), p_t, hidden_part(), h, out, a.weight_grad_type,
+                               a.accumulate != 0);
+            rc = product(n, l.seg, a.rows, grad_part(), p_t, hidden_part(), h, at(l.dw_at), SNB_TYPE_F32, false);
+            return rc != SNB_OK ? rc : store(at(l.dw_at), l.wgrad_ld, out, a.weight_grad_type, a.width, n, a.width,
+                                             a.accumulate != 0);
+        }
+        // Rows of round_up(n, 8) columns: those past n come from P's padding, are never stored, and touch no others.
+        const uint64_t cols = round_up(n, 8);
+        rc = product(l.seg, cols, a.rows, hidden_part(), h_t, grad_part(), p_n, at(l.dw_at), SNB_TYPE_F32, false);
+        return rc != SNB_OK ? rc : store(at(l.dw_at), cols, out, a.weight_grad_type, a.classes, a.width, n,
+                                         a.accumulate != 0);
+    }
+
+    int run() const {
+        int rc = SNB_OK;
+        constexpr int kLoHiHi = 1;
+        if (l.pack_hidden) {
+            rc = pack(a.hidden, a.hidden_stride, a.rows, a.width, at(l.hidden_at), l.hidden_ld, a.rows, l.seg,
+                      l.gradients ? a.targets : nullptr, l.seg, kLoHiHi);
+            if (rc != SNB_OK) return rc;
+        }
+        // Pass 1: a weight that is read in place needs no pieces here.
+        const uint64_t step = l.pack_weight ? l.piece : a.classes;
+        const void* w = nullptr;
+        for (uint64_t v0 = 0; v0 < a.classes; v0 += step) {
+            const uint64_t n = std::min(step, a.classes - v0);
+            if ((rc = weight(v0, n, &w)) != SNB_OK) return rc;
+            if ((rc = tc_vocab_product(stream, logits(v0, n, w), err)) != SNB_OK) return rc;
+        }
+        const uint64_t blocks = (a.rows + kCombineRows - 1) / kCombineRows;
+        combine_kernel<<<static_cast<unsigned>(blocks), kCombineRows * kCombineLanes, 0, stream>>>(
+            static_cast<const float2*>(at(l.partials_at)),
+            static_cast<int64_t>((a.classes + kHalfTile - 1) / kHalfTile), static_cast<int64_t>(a.rows), a.targets,
+            a.classes, static_cast<const float*>(at(l.target_at)), a.losses,
+            l.gradients ? static_cast<float2*>(at(l.stats_at)) : nullptr, a.loss_sum);
+        if ((rc = launched("combine_kernel launch", err)) != SNB_OK) return rc;
+        if (a.loss_sum != nullptr && blocks > 1) {
+            loss_sum_kernel<<<1, 1024, 0, stream>>>(a.losses, static_cast<int64_t>(a.rows), a.loss_sum);
+            if ((rc = launched("loss_sum_kernel launch", err)) != SNB_OK) return rc;
+        }
+        if (!l.gradients) return SNB_OK;
+        // Pass 2. With one piece the packed weight is still there.
+        for (uint64_t v0 = 0; v0 < a.classes; v0 += l.piece) {
+            const uint64_t n = std::min(l.piece, a.classes - v0);
+            if ((l.pieces > 1 || !l.pack_weight) && (rc = weight(v0, n, &w)) != SNB_OK) return rc;
+            VocabProduct v = logits(v0, n, w);
+            v.grad = at(l.p_at);
+            v.grad_low = const_cast<void*>(grad_part().low);
+            v.grad_ld = l.grad_ld;
+            if ((rc = tc_vocab_product(stream, v, err)) != SNB_OK) return rc;
+            if (a.weight_grad != nullptr && (rc = weight_grad(v0, n)) != SNB_OK) return rc;
+            if (a.hidden_grad != nullptr && (rc = hidden_grad(v0, n, w)) != SNB_OK) return rc;
+        }
+        return a.hidden_grad == nullptr ? SNB_OK
+                                        : store(at(l.dh_at), l.seg, a.hidden_grad, a.hidden_grad_type, a.width, a.rows,
+                                                a.width, false);
+    }
+};
+
+}  // namespace
+
+int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std::string*) {
+    *bytes = layout_of(a).bytes;
+    return SNB_OK;
+}
+
+int vocab_loss_launch(cudaStream_t stream, const snb_vocabulary_loss_args& a, bool deterministic, int sm_budget,
+                      std::string* err) {
+    if (a.rows == 0) {
+        // No row: the sum and an overwritten weight gradient are zero.
+        cudaError_t e = a.loss_sum != nullptr ? cudaMemsetAsync(a.loss_sum, 0, sizeof(float), stream) : cudaSuccess;
+        if (e == cudaSuccess && a.weight_grad != nullptr && a.accumulate == 0)
+            e = cudaMemsetAsync(a.weight_grad, 0, a.classes * a.width * (a.weight_grad_type == SNB_TYPE_BF16 ? 2 : 4),
+                                stream);
+        if (e == cudaSuccess) return SNB_OK;
+        *err = cuda_message("cudaMemsetAsync(vocabulary loss of no rows)", e);
+        return SNB_ERR_CUDA;
+    }
+    DeviceInfo dev;
+    const int rc = current_device_info(&dev, err);
+    if (rc != SNB_OK) return rc;
+    const uintptr_t base = (reinterpret_cast<uintptr_t>(a.workspace) + 255) & ~uintptr_t(255);
+    return Call{stream, a, layout_of(a), deterministic, sm_budget, dev.sm_count, reinterpret_cast<uint8_t*>(base), err}.run();
+}
+
+}  // namespace snb

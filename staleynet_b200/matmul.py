@@ -422,6 +422,80 @@ class Gpu:
                                                   _ptr(t), t.numel(), _ptr(grad_scales), _ptr(loss_sums),
                                                   _ptr(logits_grad), gt))
 
+    def _vocabulary_loss_args(self, hidden, weight, storage, d_hidden, d_weight) -> _ffi.VocabularyLossArgs:
+        """The operands' part of snb_vocabulary_loss_args: [rows, width] hidden and the weight, whose rows may be
+        strided."""
+        import torch
+
+        _require_cuda(hidden, weight, d_hidden, d_weight)
+        ty = {torch.float32: _ffi.TYPE_F32, torch.bfloat16: _ffi.TYPE_BF16}
+        transposed = storage is Storage.TRANSPOSED
+        if hidden.dim() != 2 or weight.dim() != 2 or hidden.dtype not in ty or weight.dtype != hidden.dtype:
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT,
+                           "vocabulary_cross_entropy: hidden and weight must be matrices of float32 or bfloat16")
+        rows, width = hidden.shape
+        classes = weight.shape[0 if transposed else 1]
+        if weight.shape[1 if transposed else 0] != width:
+            raise AssertionError("vocabulary_cross_entropy: weight shape")
+        a = _ffi.VocabularyLossArgs(rows=rows, width=width, classes=classes, type=ty[hidden.dtype],
+                                    weight_transposed=int(transposed))
+        for name, t in (("hidden", hidden), ("weight", weight)):
+            n, m = t.shape
+            # A matrix of one column or row has no stride to speak of in that direction.
+            if m > 1 and t.stride(1) != 1:
+                raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"vocabulary_cross_entropy: {name}'s rows must be contiguous")
+            stride = t.stride(0) if n > 1 else m
+            setattr(a, name, t.data_ptr())
+            setattr(a, name + "_len", (n - 1) * stride + m if n else 0)
+            setattr(a, name + "_stride", stride)
+        for name, grad, like in (("hidden_grad", d_hidden, hidden), ("weight_grad", d_weight, weight)):
+            if grad is None:
+                continue
+            if grad.shape != like.shape or grad.dtype not in ty or not grad.is_contiguous():
+                raise AssertionError(f"vocabulary_cross_entropy: {name} must be a dense matrix of its operand's shape")
+            setattr(a, name, grad.data_ptr())
+            setattr(a, name + "_len", grad.numel())
+            setattr(a, name + "_type", ty[grad.dtype])
+        return a
+
+    def vocabulary_cross_entropy_workspace(self, hidden, weight, *, storage: Storage = Storage.TRANSPOSED,
+                                           d_hidden=None, d_weight=None) -> int:
+        """Bytes of workspace that vocabulary_cross_entropy needs with these tensors
+        (snb_vocabulary_cross_entropy_workspace)."""
+        a = self._vocabulary_loss_args(hidden, weight, storage, d_hidden, d_weight)
+        # Set by the call itself; here they only have to pass the checks (nothing is read through them).
+        a.targets = a.losses = 16
+        a.targets_len = a.losses_len = a.rows
+        need = ctypes.c_uint64()
+        check(self.lib.snb_vocabulary_cross_entropy_workspace(ctypes.byref(a), ctypes.byref(need)))
+        return need.value
+
+    def vocabulary_cross_entropy(self, hidden, weight, targets, losses, loss_sum, workspace, *,
+                                 storage: Storage = Storage.TRANSPOSED, d_hidden=None, d_weight=None,
+                                 grad_scale: float = 1.0, write: WriteMode = WriteMode.OVERWRITE,
+                                 deterministic: bool = False) -> None:
+        """Softmax cross entropy of hidden [rows, width] over the classes of `weight`, without keeping the logits
+        (snb_vocabulary_cross_entropy): per-row losses and their sum (or None), and when given the gradients of
+        hidden and weight times grad_scale. storage: TRANSPOSED for a weight [classes, width], ROW_MAJOR for
+        [width, classes]. targets: [rows] int32, -1 (EMPTY_TOKEN) where a row has none. write: whether d_weight (f32)
+        is overwritten or added to. workspace: uint8, vocabulary_cross_entropy_workspace bytes."""
+        import torch
+
+        _require_cuda(targets, losses, loss_sum, workspace)
+        a = self._vocabulary_loss_args(hidden, weight, storage, d_hidden, d_weight)
+        if targets.dtype != torch.int32 or not targets.is_contiguous():
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: targets must be dense int32")
+        if losses.dtype != torch.float32 or (loss_sum is not None and loss_sum.dtype != torch.float32):
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: losses must be float32")
+        a.targets, a.targets_len = targets.data_ptr(), targets.numel()
+        a.losses, a.losses_len = losses.data_ptr(), losses.numel()
+        a.loss_sum = loss_sum.data_ptr() if loss_sum is not None else None
+        a.grad_scale = grad_scale
+        a.flags = _ffi.GEMM_DETERMINISTIC if deterministic else 0
+        a.accumulate = write.flag()
+        a.workspace, a.workspace_len = workspace.data_ptr(), workspace.numel() * workspace.element_size()
+        check(self.lib.snb_vocabulary_cross_entropy(self._stream_handle(), ctypes.byref(a)))
+
     def split_heads(self, packed, head_major, layout: "_ffi.HeadLayout") -> None:
         """`Gpu::split_heads` (crates/staleynet-cuda/src/ops/attention.rs:20-36): packed columns -> head-major; f32
         through snb_split_heads, other dtypes through snb_permute_heads."""
