@@ -459,6 +459,46 @@ SNB_API int snb_rms_norm_stats(void* stream, const void* input, int32_t input_ty
 SNB_API int snb_scale_rows(void* stream, const float* scale, const void* input, int32_t input_type, void* output,
                            int32_t output_type, uint64_t rows, uint64_t cols);
 
+/* Layer norm over rows of `cols` features: mean and variance of each row, y = (x - mean) * inv_std * gain + bias with
+ * inv_std = 1 / sqrt(variance + epsilon), the variance that of the row itself (divided by cols). Sums in f32. */
+typedef struct snb_layer_norm_args {
+    uint64_t rows, cols;
+    const void* input;          /* [rows, cols], rows input_stride elements apart, as every tensor here may be */
+    uint64_t input_len, input_stride;
+    int32_t input_type;         /* SNB_TYPE_* */
+    float epsilon;              /* forward; not negative */
+    const float* gain;          /* [cols] */
+    const float* bias;          /* forward: [cols] or NULL */
+    uint64_t params_len;        /* of gain, bias, gain_grad and bias_grad: cols */
+    float* mean;                /* [rows]; forward: written, backward: read */
+    float* inv_std;
+    uint64_t stats_len;         /* of both: at least rows */
+    void* output;               /* forward; may be the input itself if types and strides agree */
+    uint64_t output_len, output_stride;
+    int32_t output_type;
+    int32_t output_grad_type;
+    const void* output_grad;    /* backward */
+    uint64_t output_grad_len, output_grad_stride;
+    void* input_grad;           /* backward, of the input's type; may be output_grad itself if types and strides agree */
+    uint64_t input_grad_len, input_grad_stride;
+    float* gain_grad;           /* backward: [cols] */
+    float* bias_grad;           /* [cols] or NULL */
+    int32_t accumulate;         /* 1: gain_grad and bias_grad are added to, 0: overwritten */
+    int32_t reserved;
+    void* workspace;            /* backward: snb_layer_norm_workspace bytes, used until the call's work is done */
+    uint64_t workspace_len;
+} snb_layer_norm_args;
+
+/* *bytes = the workspace of snb_layer_norm_backward on the current device. */
+SNB_API int snb_layer_norm_workspace(uint64_t rows, uint64_t cols, uint64_t* bytes);
+
+/* Checks of both, in this order: sizes, types and strides, "params length" (params_len != cols), lengths, null and
+ * misaligned pointers, workspace. No reference counterpart (the reference normalises by the root mean square). */
+SNB_API int snb_layer_norm_forward(void* stream, const snb_layer_norm_args* args);
+
+/* input_grad, and the sums over the rows gain_grad and bias_grad, in a fixed order (the same from run to run). */
+SNB_API int snb_layer_norm_backward(void* stream, const snb_layer_norm_args* args);
+
 /* AdamWHyperparameters (ops/optimizer.rs:9-28). */
 typedef struct snb_adamw_hyper {
     float learning_rate;

@@ -74,6 +74,9 @@ EXPORTED_SYMBOLS = (
     "snb_split_heads",
     "snb_merge_heads",
     "snb_permute_heads",
+    "snb_layer_norm_workspace",
+    "snb_layer_norm_forward",
+    "snb_layer_norm_backward",
     "snb_rms_norm_forward",
     "snb_rms_norm_backward",
     "snb_rms_norm_stats",
@@ -181,6 +184,19 @@ class VocabularyLossArgs(ctypes.Structure):
                 ("accumulate", c_int32), ("reserved", c_int32), ("workspace", c_void_p), ("workspace_len", c_uint64)]
 
 
+class LayerNormArgs(ctypes.Structure):
+    """snb_layer_norm_args."""
+    _fields_ = [("rows", c_uint64), ("cols", c_uint64), ("input", c_void_p), ("input_len", c_uint64),
+                ("input_stride", c_uint64), ("input_type", c_int32), ("epsilon", c_float), ("gain", c_void_p),
+                ("bias", c_void_p), ("params_len", c_uint64), ("mean", c_void_p), ("inv_std", c_void_p),
+                ("stats_len", c_uint64), ("output", c_void_p), ("output_len", c_uint64), ("output_stride", c_uint64),
+                ("output_type", c_int32), ("output_grad_type", c_int32), ("output_grad", c_void_p),
+                ("output_grad_len", c_uint64), ("output_grad_stride", c_uint64), ("input_grad", c_void_p),
+                ("input_grad_len", c_uint64), ("input_grad_stride", c_uint64), ("gain_grad", c_void_p),
+                ("bias_grad", c_void_p), ("accumulate", c_int32), ("reserved", c_int32), ("workspace", c_void_p),
+                ("workspace_len", c_uint64)]
+
+
 assert ctypes.sizeof(Operand) == 24
 assert ctypes.sizeof(Product) == 88
 assert ctypes.sizeof(HeadLayout) == 64
@@ -251,6 +267,12 @@ def load() -> ctypes.CDLL:
         lib.snb_vocabulary_cross_entropy_workspace.restype = c_int
         lib.snb_vocabulary_cross_entropy.argtypes = [c_void_p, POINTER(VocabularyLossArgs)]
         lib.snb_vocabulary_cross_entropy.restype = c_int
+        lib.snb_layer_norm_workspace.argtypes = [c_uint64, c_uint64, POINTER(c_uint64)]
+        lib.snb_layer_norm_workspace.restype = c_int
+        lib.snb_layer_norm_forward.argtypes = [c_void_p, POINTER(LayerNormArgs)]
+        lib.snb_layer_norm_forward.restype = c_int
+        lib.snb_layer_norm_backward.argtypes = [c_void_p, POINTER(LayerNormArgs)]
+        lib.snb_layer_norm_backward.restype = c_int
         lib.snb_split_heads.argtypes = [c_void_p, c_void_p, c_uint64, c_void_p, c_uint64, POINTER(HeadLayout)]
         lib.snb_split_heads.restype = c_int
         lib.snb_merge_heads.argtypes = [c_void_p, c_void_p, c_uint64, c_void_p, c_uint64, POINTER(HeadLayout)]

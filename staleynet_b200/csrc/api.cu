@@ -608,6 +608,95 @@ int snb_vocabulary_cross_entropy(void* stream, const snb_vocabulary_loss_args* a
     return SNB_OK;
 }
 
+namespace {
+
+// One [rows, cols] tensor of a layer norm call; `what` names it in the message.
+int check_norm_tensor(const char* name, const char* what, const snb_layer_norm_args& a, const void* base, uint64_t len,
+                      uint64_t stride, int32_t type, int too_small) {
+    const std::string at = std::string(name) + ": " + what;
+    if (type != SNB_TYPE_F32 && type != SNB_TYPE_BF16) return fail(SNB_ERR_INVALID_ARGUMENT, at + " has an unknown type");
+    if (stride < a.cols || stride > (1ull << 32)) return fail(SNB_ERR_INVALID_ARGUMENT, at + " stride out of range");
+    if (a.rows == 0) return SNB_OK;
+    if (len < (a.rows - 1) * stride + a.cols) return fail(too_small, at + " too small");
+    if (base == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, at + " is null");
+    if (reinterpret_cast<uintptr_t>(base) % (type == SNB_TYPE_BF16 ? 2 : 4) != 0)
+        return fail(SNB_ERR_INVALID_ARGUMENT, at + " is not aligned to its element");
+    return SNB_OK;
+}
+
+int check_layer_norm(const char* name, const snb_layer_norm_args* a) {
+    if (a == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, std::string(name) + ": args is null");
+    const std::string n(name);
+    const uint64_t lim = (1ull << 31) - 1;
+    if (a->cols == 0 || a->cols > lim || a->rows > lim)
+        return fail(SNB_ERR_INVALID_ARGUMENT, n + ": rows or cols out of range");
+    if (a->params_len != a->cols) return fail(SNB_ERR_INVALID_ARGUMENT, n + ": params length");
+    if (a->stats_len < a->rows) return fail(SNB_ERR_INVALID_ARGUMENT, n + ": mean and inv_std too small");
+    if (a->gain == nullptr || (a->rows > 0 && (a->mean == nullptr || a->inv_std == nullptr)))
+        return fail(SNB_ERR_INVALID_ARGUMENT, n + ": null pointer");
+    for (const void* p : {static_cast<const void*>(a->gain), static_cast<const void*>(a->bias),
+                          static_cast<const void*>(a->mean), static_cast<const void*>(a->inv_std),
+                          static_cast<const void*>(a->gain_grad), static_cast<const void*>(a->bias_grad)})
+        if (reinterpret_cast<uintptr_t>(p) % 4 != 0)
+            return fail(SNB_ERR_INVALID_ARGUMENT, n + ": a pointer is not aligned to its element");
+    return check_norm_tensor(name, "input", *a, a->input, a->input_len, a->input_stride, a->input_type,
+                             SNB_ERR_INVALID_ARGUMENT);
+}
+
+}  // namespace
+
+int snb_layer_norm_workspace(uint64_t rows, uint64_t cols, uint64_t* bytes) {
+    if (bytes == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, "layer_norm_workspace: null pointer");
+    if (cols == 0 || cols >= (1ull << 31) || rows >= (1ull << 31))
+        return fail(SNB_ERR_INVALID_ARGUMENT, "layer_norm_workspace: rows or cols out of range");
+    std::string err;
+    const int rc = layer_norm_workspace(rows, cols, bytes, &err);
+    return rc == SNB_OK ? rc : fail(rc, err);
+}
+
+int snb_layer_norm_forward(void* stream, const snb_layer_norm_args* args) {
+    t_last_path = SNB_PATH_NONE;
+    const char* name = "layer_norm_forward";
+    int rc = check_layer_norm(name, args);
+    if (rc != SNB_OK) return rc;
+    if (!(args->epsilon >= 0.0f)) return fail(SNB_ERR_INVALID_ARGUMENT, "layer_norm_forward: epsilon is negative");
+    rc = check_norm_tensor(name, "output", *args, args->output, args->output_len, args->output_stride,
+                           args->output_type, SNB_ERR_OUTPUT_TOO_SMALL);
+    if (rc != SNB_OK) return rc;
+    std::string err;
+    rc = layer_norm_forward_launch(static_cast<cudaStream_t>(stream), *args, &err);
+    if (rc != SNB_OK) return fail(rc, err);
+    t_last_path = args->rows == 0 ? SNB_PATH_EMPTY : SNB_PATH_SIMT;
+    return SNB_OK;
+}
+
+int snb_layer_norm_backward(void* stream, const snb_layer_norm_args* args) {
+    t_last_path = SNB_PATH_NONE;
+    const char* name = "layer_norm_backward";
+    int rc = check_layer_norm(name, args);
+    if (rc != SNB_OK) return rc;
+    rc = check_norm_tensor(name, "output_grad", *args, args->output_grad, args->output_grad_len,
+                           args->output_grad_stride, args->output_grad_type, SNB_ERR_INVALID_ARGUMENT);
+    if (rc != SNB_OK) return rc;
+    rc = check_norm_tensor(name, "input_grad", *args, args->input_grad, args->input_grad_len, args->input_grad_stride,
+                           args->input_type, SNB_ERR_OUTPUT_TOO_SMALL);
+    if (rc != SNB_OK) return rc;
+    if (args->gain_grad == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, "layer_norm_backward: null pointer");
+    std::string err;
+    uint64_t need = 0;
+    if (args->rows > 0 && (rc = layer_norm_workspace(args->rows, args->cols, &need, &err)) != SNB_OK)
+        return fail(rc, err);
+    if (args->workspace_len < need || (need > 0 && (args->workspace == nullptr ||
+                                                    reinterpret_cast<uintptr_t>(args->workspace) % 4 != 0)))
+        return fail(SNB_ERR_INVALID_ARGUMENT, "layer_norm_backward: workspace holds " +
+                                                  std::to_string(args->workspace_len) + " bytes, needs " +
+                                                  std::to_string(need));
+    rc = layer_norm_backward_launch(static_cast<cudaStream_t>(stream), *args, &err);
+    if (rc != SNB_OK) return fail(rc, err);
+    t_last_path = args->rows == 0 ? SNB_PATH_EMPTY : SNB_PATH_SIMT;
+    return SNB_OK;
+}
+
 int snb_rms_norm_forward(void* stream, const float* input, uint64_t rows, uint64_t cols, const float* gain,
                          uint64_t gain_len, float* output, float* inv_rms, uint64_t inv_rms_len, float epsilon) {
     t_last_path = SNB_PATH_NONE;

@@ -136,6 +136,11 @@ int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std
 int vocab_loss_launch(cudaStream_t stream, const snb_vocabulary_loss_args& a, bool deterministic, int sm_budget,
                       std::string* err);
 
+// Layer norm (layer_norm.cu).
+int layer_norm_workspace(uint64_t rows, uint64_t cols, uint64_t* bytes, std::string* err);
+int layer_norm_forward_launch(cudaStream_t stream, const snb_layer_norm_args& a, std::string* err);
+int layer_norm_backward_launch(cudaStream_t stream, const snb_layer_norm_args& a, std::string* err);
+
 std::string cuda_message(const char* what, cudaError_t e);
 
 // The reference's seeded stream on the device (random.cu): normal values (f32 or bf16 output) and below(bound)
