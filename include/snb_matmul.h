@@ -535,6 +535,50 @@ SNB_API int snb_sum_of_squares(void* stream, const float* values, uint64_t count
 SNB_API int snb_adamw_step_multi(void* stream, const snb_adamw_tensor* tensors, uint64_t tensor_count,
                                  const snb_adamw_hyper* hyper, float max_gradient_norm, double* gradient_square_sum);
 
+/* One parameter tensor of snb_adamw8_step (80 bytes). Both moments are held in 8 bits: each block of 256 consecutive
+ * elements has an f32 scale S and each element a code, m = sign(q) (q / 127)^2 S and v = (q / 255)^4 S. All zeros are
+ * the moments of a first step. */
+typedef struct snb_adamw8_tensor {
+    float* parameter;
+    const void* gradient;   /* of gradient_type */
+    int8_t* first;          /* [count] codes */
+    float* first_scale;     /* [ceil(count / 256)] */
+    uint8_t* second;
+    float* second_scale;
+    uint16_t* shadow;       /* [count] receives the parameter as bf16; or NULL */
+    uint64_t count;
+    uint64_t first_draw;    /* draws of the seed's stream before this tensor's (it takes one for two elements) */
+    float weight_decay;
+    int32_t gradient_type;  /* SNB_TYPE_* */
+} snb_adamw8_tensor;
+
+/* One tensor of snb_adamw8_moments (56 bytes). */
+typedef struct snb_adamw8_moments_out {
+    const int8_t* first;
+    const float* first_scale;
+    const uint8_t* second;
+    const float* second_scale;
+    float* first_out;
+    float* second_out;
+    uint64_t count;
+} snb_adamw8_moments_out;
+
+/* Bytes of workspace of snb_adamw8_step. */
+SNB_API uint64_t snb_adamw8_workspace(uint64_t tensor_count);
+
+/* snb_adamw_step_multi for moments in 8 bits and any number of tensors: the update on the values that the codes stand
+ * for, the new moments rounded to one of the two levels around them with the probability that keeps their expectation.
+ * The draws are those of the reference's generator with `seed` (snb_random_normal's), which has to be another one in each
+ * step: output first_draw + i + 1 serves elements 2i and 2i + 1 of a tensor. A gradient that is not finite makes its
+ * block's moments NaN. max_gradient_norm may be infinite. The same inputs give the same bits. No reference counterpart
+ * (the reference keeps 32-bit moments). */
+SNB_API int snb_adamw8_step(void* stream, const snb_adamw8_tensor* tensors, uint64_t tensor_count,
+                            const snb_adamw_hyper* hyper, float max_gradient_norm, uint64_t seed,
+                            double* gradient_square_sum, void* workspace, uint64_t workspace_len);
+
+/* The f32 values of both moments of every tensor. */
+SNB_API int snb_adamw8_moments(void* stream, const snb_adamw8_moments_out* tensors, uint64_t tensor_count);
+
 /* Seeded inputs on the device, the reference's generator (`Random`, crates/staleynet-model/src/random.rs:27-70):
  * SplitMix64 whose k-th draw (k = 1, 2, ...) from Random::new(seed) is its output for state seed + k * 0x9E3779B97F4A7C15.
  * output[i] = std * normal() computed from draws first_draw + 2i + 1 and + 2 (random.rs:64-68, two draws per value),

@@ -84,6 +84,9 @@ EXPORTED_SYMBOLS = (
     "snb_adamw_step",
     "snb_sum_of_squares",
     "snb_adamw_step_multi",
+    "snb_adamw8_workspace",
+    "snb_adamw8_step",
+    "snb_adamw8_moments",
     "snb_random_normal",
     "snb_random_below",
     "snb_selftest_bounded_wait",
@@ -124,6 +127,19 @@ class AdamWTensor(ctypes.Structure):
     """snb_adamw_tensor."""
     _fields_ = [("parameter", c_void_p), ("gradient", c_void_p), ("first_moment", c_void_p),
                 ("second_moment", c_void_p), ("count", c_uint64), ("weight_decay", c_float), ("reserved", c_uint32)]
+
+
+class AdamW8Tensor(ctypes.Structure):
+    """snb_adamw8_tensor."""
+    _fields_ = [("parameter", c_void_p), ("gradient", c_void_p), ("first", c_void_p), ("first_scale", c_void_p),
+                ("second", c_void_p), ("second_scale", c_void_p), ("shadow", c_void_p), ("count", c_uint64),
+                ("first_draw", c_uint64), ("weight_decay", c_float), ("gradient_type", c_int32)]
+
+
+class AdamW8Moments(ctypes.Structure):
+    """snb_adamw8_moments_out."""
+    _fields_ = [("first", c_void_p), ("first_scale", c_void_p), ("second", c_void_p), ("second_scale", c_void_p),
+                ("first_out", c_void_p), ("second_out", c_void_p), ("count", c_uint64)]
 
 
 class HeadLayout(ctypes.Structure):
@@ -273,6 +289,13 @@ def load() -> ctypes.CDLL:
         lib.snb_layer_norm_forward.restype = c_int
         lib.snb_layer_norm_backward.argtypes = [c_void_p, POINTER(LayerNormArgs)]
         lib.snb_layer_norm_backward.restype = c_int
+        lib.snb_adamw8_workspace.argtypes = [c_uint64]
+        lib.snb_adamw8_workspace.restype = c_uint64
+        lib.snb_adamw8_step.argtypes = [c_void_p, POINTER(AdamW8Tensor), c_uint64, POINTER(AdamWHyper), c_float, c_uint64,
+                                        c_void_p, c_void_p, c_uint64]
+        lib.snb_adamw8_step.restype = c_int
+        lib.snb_adamw8_moments.argtypes = [c_void_p, POINTER(AdamW8Moments), c_uint64]
+        lib.snb_adamw8_moments.restype = c_int
         lib.snb_split_heads.argtypes = [c_void_p, c_void_p, c_uint64, c_void_p, c_uint64, POINTER(HeadLayout)]
         lib.snb_split_heads.restype = c_int
         lib.snb_merge_heads.argtypes = [c_void_p, c_void_p, c_uint64, c_void_p, c_uint64, POINTER(HeadLayout)]

@@ -1,0 +1,453 @@
+// adamw8.cu — an AdamW step over many tensors with both moments held in 8 bits.
+//
+// Moments. A block of 256 consecutive elements of a tensor shares an f32 scale S for each moment, the largest magnitude
+// in the block, and each element an 8-bit code: m = sign(q) (q / 127)^2 S with q in -127 .. 127, v = (q / 255)^4 S with q
+// in 0 .. 255. The levels are powers because a block's gradients differ by orders of magnitude: equal steps would leave
+// nothing of the small ones, while here the steps near a value x of the block shrink like sqrt(x) and x^(3/4).
+//   A value between two levels goes to the upper one with the probability that keeps its expectation, drawn from a
+// caller's seed. Rounding to nearest instead would freeze v: with beta2 = 0.999 a step moves it by a thousandth, and
+// neighbouring levels are 1.6 % apart or more. A v above 0 keeps at least code 1: a v of 0 next to an m that is not
+// would divide that m by epsilon.
+//   The random bits of elements 2i and 2i + 1 of a tensor are the halves of output first_draw + i + 1 of the reference's
+// SplitMix64 (Random::new(seed), crates/staleynet-model/src/random.rs:27-50): 16 bits for each moment.
+//   Everything that decides a code is written with explicitly rounded f32 operations, so codes do not depend on how the
+// compiler contracts them.
+//
+// Step. As the reference's (kernels/optimizer.rs:57-70) on g = gradient times the clip factor max_norm / norm; the norm is
+// that of all tensors together, its squares summed in f64 in a fixed order, so steps are the same from run to run.
+//
+// What bounds it: memory. An element's parameter (4 bytes read, 4 written, and 2 for its bf16 copy), gradient (2 or 4,
+// twice: once for the norm) and two codes (2 read, 2 written).
+#include <cuda_runtime.h>
+
+#include <algorithm>
+#include <cmath>
+#include <cstdint>
+#include <string>
+
+#include "internal.h"
+
+namespace snb {
+namespace {
+
+constexpr int kBlock = 256;             // elements that share a scale
+constexpr int kWarps = 8;               // warps of a thread block
+constexpr int kChunk = 4 * kWarps * kBlock;  // elements that a thread block takes at a time
+constexpr int kMaxTensors = 256;        // of one launch (its table is a kernel parameter)
+constexpr int kSumBlocks = 592;         // thread blocks of the norm's sum, and partial sums of one launch
+constexpr uint64_t kGolden = 0x9E3779B97F4A7C15ull;
+
+struct Table {
+    int32_t n;
+    snb_adamw8_tensor t[kMaxTensors];
+    int64_t chunk_start[kMaxTensors + 1];
+};
+static_assert(sizeof(Table) < 32000, "kernel parameters");
+
+__device__ __forceinline__ int tensor_of_chunk(const int64_t* chunk_start, int n, int64_t chunk) {
+    int lo = 0, hi = n - 1;
+    while (lo < hi) {  // last tensor that starts at or before the chunk (an empty one starts where the next does)
+        const int mid = (lo + hi + 1) >> 1;
+        if (chunk_start[mid] <= chunk) lo = mid;
+        else hi = mid - 1;
+    }
+    return lo;
+}
+
+__device__ __forceinline__ float bf16_value(uint16_t h) { return __uint_as_float(static_cast<uint32_t>(h) << 16); }
+
+__device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
+    uint32_t r;
+    asm("cvt.rn.bf16x2.f32 %0, %1, %2;" : "=r"(r) : "f"(hi), "f"(lo));
+    return r;
+}
+
+__device__ __forceinline__ bool multiple(const void* p, uint32_t n) {
+    return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
+}
+
+// The share of its block's scale that a magnitude code stands for.
+__device__ __forceinline__ float first_level(float q) { return __fmul_rn(__fmul_rn(q, q), 1.0f / 16129.0f); }
+__device__ __forceinline__ float second_level(float q) {
+    const float s = __fmul_rn(__fmul_rn(q, q), 1.0f / 65025.0f);
+    return __fmul_rn(s, s);
+}
+
+__device__ __forceinline__ float sqrt_fast(float x) {
+    float y;
+    asm("sqrt.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
+}
+
+// The code of `share` (a magnitude over its block's scale): q is the last level up to it, found from `guess`, which may
+// be one level off, and kept below the last level; the upper neighbour is taken if the random threshold between the two
+// lies below the share. NaN gives 0.
+template <typename Level>
+__device__ __forceinline__ float encode(float share, float guess, float most, uint32_t bits16, Level level) {
+    float q = share > 0.0f ? fminf(floorf(guess), most - 1.0f) : 0.0f;
+    float low = level(q), high = level(q + 1.0f);
+    if (low > share && q > 0.0f) {
+        q -= 1.0f;
+        high = low;
+        low = level(q);
+    } else if (high <= share && q < most - 1.0f) {
+        q += 1.0f;
+        low = high;
+        high = level(q + 1.0f);
+    }
+    const float u = __fmul_rn(__fadd_rn(static_cast<float>(bits16), 0.5f), 1.0f / 65536.0f);
+    const float threshold = __fadd_rn(low, __fmul_rn(u, __fsub_rn(high, low)));
+    return threshold < share ? q + 1.0f : q;
+}
+
+// (scale, 1 / scale) of a block whose largest magnitude has these bits (as integers magnitudes order like floats, with
+// infinity and NaN above all others: a block that holds one decodes to NaN). Subnormal scales count as 0.
+__device__ __forceinline__ float2 scale_of(uint32_t bits) {
+    const float s = __uint_as_float(bits);
+    if (s < 1.17549435e-38f) return make_float2(0.0f, 0.0f);
+    return make_float2(s, s > 0.0f ? __frcp_rn(s) : 0.0f);
+}
+
+// SplitMix64's output for a state.
+__device__ __forceinline__ uint64_t mix(uint64_t z) {
+    z = (z ^ (z >> 30)) * 0xBF58476D1CE4E5B9ull;
+    z = (z ^ (z >> 27)) * 0x94D049BB133111EBull;
+    return z ^ (z >> 31);
+}
+
+// A lane's elements of a block: 4 from 4 * lane and 4 from 128 + 4 * lane, so that every access of a warp is contiguous.
+__device__ __forceinline__ int element_of(int lane, int j) { return (j >> 2) * 128 + 4 * lane + (j & 3); }
+
+// The f64 sum of v over the thread block, in every thread, in a fixed order.
+__device__ __forceinline__ double block_sum(double v) {
+    __shared__ double part[kWarps];
+#pragma unroll
+    for (int s = 16; s > 0; s >>= 1) v += __shfl_xor_sync(0xffffffffu, v, s);
+    __syncthreads();
+    if ((threadIdx.x & 31) == 0) part[threadIdx.x >> 5] = v;
+    __syncthreads();
+    double sum = 0.0;
+    for (int w = 0; w < kWarps; ++w) sum += part[w];
+    return sum;
+}
+
+__global__ void __launch_bounds__(32 * kWarps) adamw8_norm_kernel(const __grid_constant__ Table m, double* partials) {
+    const int64_t chunks = m.chunk_start[m.n];
+    double sum = 0.0;
+    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int t = tensor_of_chunk(m.chunk_start, m.n, chunk);
+        const snb_adamw8_tensor& x = m.t[t];
+        const int64_t begin = (chunk - m.chunk_start[t]) * kChunk;
+        const int64_t n = min(static_cast<int64_t>(x.count) - begin, static_cast<int64_t>(kChunk));
+        const bool bf16 = x.gradient_type == SNB_TYPE_BF16;
+        int64_t scalar_begin = 0;
+        if (bf16 && multiple(x.gradient, 16)) {
+            const uint4* g = reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(x.gradient) + begin);
+            for (int64_t i = threadIdx.x; i < n / 8; i += 32 * kWarps) {
+                const uint4 q = __ldg(g + i);
+                for (uint32_t w : {q.x, q.y, q.z, q.w}) {
+                    const double lo = __uint_as_float(w << 16), hi = __uint_as_float(w & 0xFFFF0000u);
+                    sum += lo * lo;
+                    sum += hi * hi;
+                }
+            }
+            scalar_begin = n / 8 * 8;
+        } else if (!bf16 && multiple(x.gradient, 16)) {
+            const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(x.gradient) + begin);
+#pragma unroll 4
+            for (int64_t i = threadIdx.x; i < n / 4; i += 32 * kWarps) {
+                const float4 q = __ldg(g + i);
+                for (double v : {static_cast<double>(q.x), static_cast<double>(q.y), static_cast<double>(q.z),
+                                 static_cast<double>(q.w)})
+                    sum += v * v;
+            }
+            scalar_begin = n / 4 * 4;
+        }
+        for (int64_t i = scalar_begin + threadIdx.x; i < n; i += 32 * kWarps) {
+            const double v = bf16 ? bf16_value(static_cast<const uint16_t*>(x.gradient)[begin + i])
+                                  : static_cast<const float*>(x.gradient)[begin + i];
+            sum += v * v;
+        }
+    }
+    sum = block_sum(sum);
+    if (threadIdx.x == 0) partials[blockIdx.x] = sum;
+}
+
+struct StepParams {
+    float learning_rate, beta1, beta2, one_minus_beta1, one_minus_beta2, epsilon;
+    float first_correction, second_correction;  // 1 / (1 - beta^step)
+    float max_norm;
+    uint64_t seed;
+    const double* partials;
+    int32_t partial_count;
+    double* square_sum;
+};
+
+__global__ void __launch_bounds__(32 * kWarps) adamw8_step_kernel(const __grid_constant__ Table m, const StepParams a) {
+    // Every thread block adds the norm's partial sums in the same order.
+    double sum = 0.0;
+    for (int i = threadIdx.x; i < a.partial_count; i += 32 * kWarps) sum += a.partials[i];
+    sum = block_sum(sum);
+    if (blockIdx.x == 0 && threadIdx.x == 0) *a.square_sum = sum;
+    const float norm = static_cast<float>(sqrt(sum));
+    const float clip = norm > a.max_norm ? __fdiv_rn(a.max_norm, norm) : 1.0f;
+
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t chunks = m.chunk_start[m.n];
+    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int t = tensor_of_chunk(m.chunk_start, m.n, chunk);
+        const snb_adamw8_tensor& x = m.t[t];
+        const int64_t begin = (chunk - m.chunk_start[t]) * kChunk;
+        const int64_t count = static_cast<int64_t>(x.count);
+        const bool grad_bf16 = x.gradient_type == SNB_TYPE_BF16;
+        const bool aligned = multiple(x.parameter, 16) && multiple(x.gradient, grad_bf16 ? 8 : 16) &&
+                             multiple(x.first, 4) && multiple(x.second, 4) && multiple(x.shadow, 8);
+        for (int64_t at = begin + warp * kBlock; at < min(begin + kChunk, count); at += kWarps * kBlock) {
+            const bool whole = aligned && at + kBlock <= count;
+            float w[8], g[8];
+            uint32_t c1[2] = {0, 0}, c2[2] = {0, 0};
+            if (whole) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t e = at + element_of(lane, 4 * h);
+                    const float4 wv = *reinterpret_cast<const float4*>(x.parameter + e);
+                    w[4 * h] = wv.x; w[4 * h + 1] = wv.y; w[4 * h + 2] = wv.z; w[4 * h + 3] = wv.w;
+                    if (grad_bf16) {
+                        const uint2 q = __ldg(reinterpret_cast<const uint2*>(static_cast<const uint16_t*>(x.gradient) + e));
+                        g[4 * h] = __uint_as_float(q.x << 16); g[4 * h + 1] = __uint_as_float(q.x & 0xFFFF0000u);
+                        g[4 * h + 2] = __uint_as_float(q.y << 16); g[4 * h + 3] = __uint_as_float(q.y & 0xFFFF0000u);
+                    } else {
+                        const float4 q = __ldg(reinterpret_cast<const float4*>(static_cast<const float*>(x.gradient) + e));
+                        g[4 * h] = q.x; g[4 * h + 1] = q.y; g[4 * h + 2] = q.z; g[4 * h + 3] = q.w;
+                    }
+                    c1[h] = *reinterpret_cast<const uint32_t*>(x.first + e);
+                    c2[h] = *reinterpret_cast<const uint32_t*>(x.second + e);
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t e = at + element_of(lane, j);
+                    const bool live = e < count;
+                    w[j] = live ? x.parameter[e] : 0.0f;
+                    g[j] = !live ? 0.0f
+                                 : grad_bf16 ? bf16_value(static_cast<const uint16_t*>(x.gradient)[e])
+                                             : static_cast<const float*>(x.gradient)[e];
+                    const uint32_t b1 = live ? static_cast<uint8_t>(x.first[e]) : 0, b2 = live ? x.second[e] : 0;
+                    c1[j >> 2] |= b1 << (8 * (j & 3));
+                    c2[j >> 2] |= b2 << (8 * (j & 3));
+                }
+            }
+            const float s1 = x.first_scale[at / kBlock], s2 = x.second_scale[at / kBlock];
+            float mean[8], variance[8];
+            uint32_t top1 = 0, top2 = 0;
+#pragma unroll
+            for (int j = 0; j < 8; ++j) {
+                const float q1 = static_cast<float>(static_cast<int8_t>(c1[j >> 2] >> (8 * (j & 3))));
+                const float q2 = static_cast<float>((c2[j >> 2] >> (8 * (j & 3))) & 0xFFu);
+                const float gj = __fmul_rn(g[j], clip);
+                const float old1 = __fmul_rn(__fmul_rn(__fmul_rn(q1, fabsf(q1)), 1.0f / 16129.0f), s1);
+                const float old2 = __fmul_rn(second_level(q2), s2);
+                mean[j] = __fadd_rn(__fmul_rn(old1, a.beta1), __fmul_rn(gj, a.one_minus_beta1));
+                variance[j] = __fadd_rn(__fmul_rn(old2, a.beta2), __fmul_rn(__fmul_rn(gj, a.one_minus_beta2), gj));
+                top1 = max(top1, __float_as_uint(mean[j]) & 0x7FFFFFFFu);
+                top2 = max(top2, __float_as_uint(variance[j]) & 0x7FFFFFFFu);
+                // The update itself decides no code: approximate root and quotient (2^-22) far below its own step.
+                const float root = sqrt_fast(variance[j] * a.second_correction) + a.epsilon;
+                const float update = __fdividef(mean[j] * a.first_correction, root) + x.weight_decay * w[j];
+                w[j] -= a.learning_rate * update;
+            }
+            const float2 n1 = scale_of(__reduce_max_sync(0xffffffffu, top1));
+            const float2 n2 = scale_of(__reduce_max_sync(0xffffffffu, top2));
+            c1[0] = c1[1] = c2[0] = c2[1] = 0;
+#pragma unroll
+            for (int j = 0; j < 8; j += 2) {
+                const uint64_t draw = x.first_draw + static_cast<uint64_t>(at + element_of(lane, j)) / 2 + 1;
+                const uint64_t bits = mix(a.seed + draw * kGolden);
+#pragma unroll
+                for (int k = 0; k < 2; ++k) {
+                    const uint32_t b = static_cast<uint32_t>(bits >> (32 * k));
+                    const float share1 = __fmul_rn(fabsf(mean[j + k]), n1.y);
+                    const float share2 = __fmul_rn(variance[j + k], n2.y);
+                    const float q1 = encode(share1, 127.0f * sqrt_fast(share1), 127.0f, b & 0xFFFFu, first_level);
+                    float q2 = encode(share2, 255.0f * sqrt_fast(sqrt_fast(share2)), 255.0f, b >> 16, second_level);
+                    if (variance[j + k] > 0.0f) q2 = fmaxf(q2, 1.0f);
+                    const int code1 = mean[j + k] < 0.0f ? -static_cast<int>(q1) : static_cast<int>(q1);
+                    const int shift = 8 * ((j + k) & 3);
+                    c1[j >> 2] |= (static_cast<uint32_t>(code1) & 0xFFu) << shift;
+                    c2[j >> 2] |= static_cast<uint32_t>(q2) << shift;
+                }
+            }
+            if (lane == 0) {
+                x.first_scale[at / kBlock] = n1.x;
+                x.second_scale[at / kBlock] = n2.x;
+            }
+            if (whole) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t e = at + element_of(lane, 4 * h);
+                    *reinterpret_cast<float4*>(x.parameter + e) = make_float4(w[4 * h], w[4 * h + 1], w[4 * h + 2],
+                                                                              w[4 * h + 3]);
+                    if (x.shadow != nullptr)
+                        *reinterpret_cast<uint2*>(x.shadow + e) = make_uint2(bf16_pair(w[4 * h], w[4 * h + 1]),
+                                                                             bf16_pair(w[4 * h + 2], w[4 * h + 3]));
+                    *reinterpret_cast<uint32_t*>(x.first + e) = c1[h];
+                    *reinterpret_cast<uint32_t*>(x.second + e) = c2[h];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t e = at + element_of(lane, j);
+                    if (e >= count) continue;
+                    x.parameter[e] = w[j];
+                    if (x.shadow != nullptr) x.shadow[e] = static_cast<uint16_t>(bf16_pair(w[j], 0.0f));
+                    x.first[e] = static_cast<int8_t>(c1[j >> 2] >> (8 * (j & 3)));
+                    x.second[e] = static_cast<uint8_t>(c2[j >> 2] >> (8 * (j & 3)));
+                }
+            }
+        }
+    }
+}
+
+// The moments' values in f32, for checkpoints and inspection.
+struct MomentTable {
+    int32_t n;
+    snb_adamw8_moments_out t[kMaxTensors];
+    int64_t chunk_start[kMaxTensors + 1];
+};
+static_assert(sizeof(MomentTable) < 32000, "kernel parameters");
+
+__global__ void __launch_bounds__(32 * kWarps) adamw8_moments_kernel(const __grid_constant__ MomentTable m) {
+    const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
+    const int64_t chunks = m.chunk_start[m.n];
+    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
+        const int t = tensor_of_chunk(m.chunk_start, m.n, chunk);
+        const snb_adamw8_moments_out& x = m.t[t];
+        const int64_t begin = (chunk - m.chunk_start[t]) * kChunk;
+        const int64_t count = static_cast<int64_t>(x.count);
+        const bool aligned = multiple(x.first, 4) && multiple(x.second, 4) && multiple(x.first_out, 16) &&
+                             multiple(x.second_out, 16);
+        for (int64_t at = begin + warp * kBlock; at < min(begin + kChunk, count); at += kWarps * kBlock) {
+            const float s1 = x.first_scale[at / kBlock], s2 = x.second_scale[at / kBlock];
+            auto value1 = [&](int8_t c) {
+                const float q = static_cast<float>(c);
+                return __fmul_rn(__fmul_rn(__fmul_rn(q, fabsf(q)), 1.0f / 16129.0f), s1);
+            };
+            auto value2 = [&](uint32_t c) { return __fmul_rn(second_level(static_cast<float>(c)), s2); };
+            if (aligned && at + kBlock <= count) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t e = at + element_of(lane, 4 * h);
+                    const uint32_t c1 = *reinterpret_cast<const uint32_t*>(x.first + e);
+                    const uint32_t c2 = *reinterpret_cast<const uint32_t*>(x.second + e);
+                    *reinterpret_cast<float4*>(x.first_out + e) =
+                        make_float4(value1(static_cast<int8_t>(c1)), value1(static_cast<int8_t>(c1 >> 8)),
+                                    value1(static_cast<int8_t>(c1 >> 16)), value1(static_cast<int8_t>(c1 >> 24)));
+                    *reinterpret_cast<float4*>(x.second_out + e) =
+                        make_float4(value2(c2 & 0xFFu), value2((c2 >> 8) & 0xFFu), value2((c2 >> 16) & 0xFFu),
+                                    value2(c2 >> 24));
+                }
+            } else {
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t e = at + element_of(lane, j);
+                    if (e >= count) continue;
+                    x.first_out[e] = value1(x.first[e]);
+                    x.second_out[e] = value2(x.second[e]);
+                }
+            }
+        }
+    }
+}
+
+int launched(const char* what, std::string* err) {
+    const cudaError_t e = cudaGetLastError();
+    if (e == cudaSuccess) return SNB_OK;
+    *err = cuda_message(what, e);
+    return SNB_ERR_CUDA;
+}
+
+// The table of tensors [first, first + up to kMaxTensors); returns how many it holds.
+template <typename T, typename Source>
+uint64_t fill(T* table, const Source* tensors, uint64_t first, uint64_t n) {
+    const uint64_t take = std::min<uint64_t>(n - first, kMaxTensors);
+    int64_t chunks = 0;
+    for (uint64_t i = 0; i < take; ++i) {
+        table->t[i] = tensors[first + i];
+        table->chunk_start[i] = chunks;
+        chunks += static_cast<int64_t>((tensors[first + i].count + kChunk - 1) / kChunk);
+    }
+    table->chunk_start[take] = chunks;
+    table->n = static_cast<int32_t>(take);
+    return take;
+}
+
+}  // namespace
+
+uint64_t adamw8_workspace(uint64_t tensor_count) {
+    const uint64_t launches = (tensor_count + kMaxTensors - 1) / kMaxTensors;
+    return std::max<uint64_t>(1, launches) * kSumBlocks * sizeof(double);
+}
+
+int adamw8_step_launch(cudaStream_t s, const snb_adamw8_tensor* tensors, uint64_t n, const snb_adamw_hyper& h,
+                       float max_gradient_norm, uint64_t seed, double* square_sum, double* partials, std::string* err) {
+    DeviceInfo dev;
+    int rc = current_device_info(&dev, err);
+    if (rc != SNB_OK) return rc;
+    Table table{};
+    int32_t sums = 0;
+    for (uint64_t i = 0; i < n; i += kMaxTensors) {
+        fill(&table, tensors, i, n);
+        const int64_t chunks = table.chunk_start[table.n];
+        if (chunks == 0) continue;
+        const int blocks = static_cast<int>(std::min<int64_t>(chunks, kSumBlocks));
+        adamw8_norm_kernel<<<blocks, 32 * kWarps, 0, s>>>(table, partials + sums);
+        if ((rc = launched("adamw8_norm_kernel launch", err)) != SNB_OK) return rc;
+        sums += blocks;
+    }
+    if (sums == 0) {
+        const cudaError_t e = cudaMemsetAsync(square_sum, 0, sizeof(double), s);
+        if (e == cudaSuccess) return SNB_OK;
+        *err = cuda_message("cudaMemsetAsync(gradient square sum)", e);
+        return SNB_ERR_CUDA;
+    }
+    StepParams a{};
+    a.learning_rate = h.learning_rate;
+    a.beta1 = h.beta1;
+    a.beta2 = h.beta2;
+    a.one_minus_beta1 = 1.0f - h.beta1;
+    a.one_minus_beta2 = 1.0f - h.beta2;
+    a.epsilon = h.epsilon;
+    a.first_correction = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(h.beta1), h.step)));
+    a.second_correction = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(h.beta2), h.step)));
+    a.max_norm = max_gradient_norm;
+    a.seed = seed;
+    a.partials = partials;
+    a.partial_count = sums;
+    a.square_sum = square_sum;
+    for (uint64_t i = 0; i < n; i += kMaxTensors) {
+        if (n > kMaxTensors) fill(&table, tensors, i, n);
+        const int64_t chunks = table.chunk_start[table.n];
+        if (chunks == 0) continue;
+        const int64_t blocks = std::min<int64_t>(chunks, 4ll * dev.sm_count);
+        adamw8_step_kernel<<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(table, a);
+        if ((rc = launched("adamw8_step_kernel launch", err)) != SNB_OK) return rc;
+    }
+    return SNB_OK;
+}
+
+int adamw8_moments_launch(cudaStream_t s, const snb_adamw8_moments_out* tensors, uint64_t n, std::string* err) {
+    DeviceInfo dev;
+    int rc = current_device_info(&dev, err);
+    if (rc != SNB_OK) return rc;
+    MomentTable table{};
+    for (uint64_t i = 0; i < n; i += kMaxTensors) {
+        fill(&table, tensors, i, n);
+        const int64_t chunks = table.chunk_start[table.n];
+        if (chunks == 0) continue;
+        const int64_t blocks = std::min<int64_t>(chunks, 8ll * dev.sm_count);
+        adamw8_moments_kernel<<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(table);
+        if ((rc = launched("adamw8_moments_kernel launch", err)) != SNB_OK) return rc;
+    }
+    return SNB_OK;
+}
+
+}  // namespace snb

@@ -834,6 +834,66 @@ int snb_adamw_step_multi(void* stream, const snb_adamw_tensor* tensors, uint64_t
     return SNB_OK;
 }
 
+uint64_t snb_adamw8_workspace(uint64_t tensor_count) { return adamw8_workspace(tensor_count); }
+
+int snb_adamw8_step(void* stream, const snb_adamw8_tensor* tensors, uint64_t tensor_count, const snb_adamw_hyper* hyper,
+                    float max_gradient_norm, uint64_t seed, double* gradient_square_sum, void* workspace,
+                    uint64_t workspace_len) {
+    t_last_path = SNB_PATH_NONE;
+    if (hyper == nullptr || gradient_square_sum == nullptr || (tensor_count > 0 && tensors == nullptr))
+        return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: null pointer");
+    if (tensor_count > (1ull << 20)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: too many tensors");
+    for (uint64_t i = 0; i < tensor_count; ++i) {
+        const snb_adamw8_tensor& t = tensors[i];
+        const std::string at = " in tensor " + std::to_string(i);
+        if (t.gradient_type != SNB_TYPE_F32 && t.gradient_type != SNB_TYPE_BF16)
+            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: unknown gradient type" + at);
+        if (t.count > (1ull << 40)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: too many elements" + at);
+        if (t.count > 0 && (t.parameter == nullptr || t.gradient == nullptr || t.first == nullptr ||
+                            t.first_scale == nullptr || t.second == nullptr || t.second_scale == nullptr))
+            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: null pointer" + at);
+        const uint64_t words = reinterpret_cast<uintptr_t>(t.parameter) | reinterpret_cast<uintptr_t>(t.first_scale) |
+                               reinterpret_cast<uintptr_t>(t.second_scale) |
+                               (t.gradient_type == SNB_TYPE_F32 ? reinterpret_cast<uintptr_t>(t.gradient) : 0);
+        const uint64_t halves = reinterpret_cast<uintptr_t>(t.gradient) | reinterpret_cast<uintptr_t>(t.shadow);
+        if (words % 4 != 0 || halves % 2 != 0)
+            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: a pointer is not aligned to its element" + at);
+    }
+    if (!(max_gradient_norm > 0.0f)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: max_gradient_norm <= 0");
+    if (hyper->step == 0) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: steps count from 1");
+    const uint64_t need = adamw8_workspace(tensor_count);
+    if (workspace == nullptr || workspace_len < need || reinterpret_cast<uintptr_t>(workspace) % 8 != 0)
+        return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: workspace holds " + std::to_string(workspace_len) +
+                                                  " bytes, needs " + std::to_string(need) + " on an 8-byte boundary");
+    std::string err;
+    const int rc = adamw8_step_launch(static_cast<cudaStream_t>(stream), tensors, tensor_count, *hyper, max_gradient_norm,
+                                      seed, gradient_square_sum, static_cast<double*>(workspace), &err);
+    if (rc != SNB_OK) return fail(rc, err);
+    t_last_path = SNB_PATH_SIMT;
+    return SNB_OK;
+}
+
+int snb_adamw8_moments(void* stream, const snb_adamw8_moments_out* tensors, uint64_t tensor_count) {
+    t_last_path = SNB_PATH_NONE;
+    if (tensor_count > 0 && tensors == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: null pointer");
+    for (uint64_t i = 0; i < tensor_count; ++i) {
+        const snb_adamw8_moments_out& t = tensors[i];
+        const std::string at = " in tensor " + std::to_string(i);
+        if (t.count > (1ull << 40)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: too many elements" + at);
+        if (t.count > 0 && (t.first == nullptr || t.first_scale == nullptr || t.second == nullptr ||
+                            t.second_scale == nullptr || t.first_out == nullptr || t.second_out == nullptr))
+            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: null pointer" + at);
+        if ((reinterpret_cast<uintptr_t>(t.first_scale) | reinterpret_cast<uintptr_t>(t.second_scale) |
+             reinterpret_cast<uintptr_t>(t.first_out) | reinterpret_cast<uintptr_t>(t.second_out)) % 4 != 0)
+            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: a pointer is not aligned to its element" + at);
+    }
+    std::string err;
+    const int rc = adamw8_moments_launch(static_cast<cudaStream_t>(stream), tensors, tensor_count, &err);
+    if (rc != SNB_OK) return fail(rc, err);
+    t_last_path = SNB_PATH_SIMT;
+    return SNB_OK;
+}
+
 int snb_selftest_bounded_wait(void* stream, uint64_t limit_ns) {
     if (limit_ns == 0 || limit_ns > 1000000000ull)
         return fail(SNB_ERR_INVALID_ARGUMENT, "selftest: limit_ns must lie in (0, 1 s]");

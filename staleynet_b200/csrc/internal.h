@@ -141,6 +141,12 @@ int layer_norm_workspace(uint64_t rows, uint64_t cols, uint64_t* bytes, std::str
 int layer_norm_forward_launch(cudaStream_t stream, const snb_layer_norm_args& a, std::string* err);
 int layer_norm_backward_launch(cudaStream_t stream, const snb_layer_norm_args& a, std::string* err);
 
+// AdamW with 8-bit moments (adamw8.cu).
+uint64_t adamw8_workspace(uint64_t tensor_count);
+int adamw8_step_launch(cudaStream_t stream, const snb_adamw8_tensor* tensors, uint64_t n, const snb_adamw_hyper& h,
+                       float max_gradient_norm, uint64_t seed, double* square_sum, double* partials, std::string* err);
+int adamw8_moments_launch(cudaStream_t stream, const snb_adamw8_moments_out* tensors, uint64_t n, std::string* err);
+
 std::string cuda_message(const char* what, cudaError_t e);
 
 // The reference's seeded stream on the device (random.cu): normal values (f32 or bf16 output) and below(bound)
