@@ -3,12 +3,13 @@
 //   mu = mean(x),  s = 1 / sqrt(mean((x - mu)^2) + epsilon),  y = (x - mu) s g + b                       (each row)
 //   n = (x - mu) s,  d = dy g:  dx = s (d - mean(d) - n mean(d n));  dg = sum_rows dy n,  db = sum_rows dy
 //
-// Both passes are bound by memory (x and y once; x, dy and dx once), so a row is read once and held in registers: by a
-// warp up to 1,024 columns, else by a block (Shape below). The variance is taken from the deviations, not from the
-// squares, whose difference would lose what a mean far from zero leaves. The backward pass runs a fixed grid whose warps
-// or blocks walk over the rows; each thread always has the same columns, so it keeps their dg and db sums in registers, and a second kernel adds the grid's sums in a fixed order (no
-// atomics: gradients are the same from run to run). Rows too long for that are read again instead (the wide kernels).
-// All sums are f32.
+// Both passes are bound by memory (x and y once; x, dy and dx once), so a row is read once, asynchronously into shared
+// memory, several rows ahead of the one at hand, and held in registers by a warp or, if long, by a block (Shape below). A
+// fixed grid walks over the rows: the gain and bias stay in registers, and in the backward pass so do each thread's sums
+// of dg and db, since it always has the same columns. A second kernel adds the grid's sums in a fixed order (no atomics:
+// gradients are the same from run to run). The variance is taken from the deviations, not from the squares, whose
+// difference would lose what a mean far from zero leaves. Rows too long for registers are read again instead (the wide
+// kernels). All sums are f32.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -23,55 +24,24 @@ namespace {
 
 constexpr int kWarpsPerBlock = 8;
 
-// One thread's 8 elements of a row: as they lie in memory (VEC: 16 bytes of bf16 or 32 of f32), or read one by one.
-struct Raw {
-    uint32_t w[8];
-};
-
-// Column of element e of piece v of thread t. VEC: 8 consecutive columns a thread (one or two 16-byte accesses); else
-// neighbouring threads take neighbouring columns, which coalesces single elements of rows that start anywhere.
-template <int T, bool VEC>
-__device__ __forceinline__ int64_t column(int t, int v, int e) {
-    return VEC ? static_cast<int64_t>(v * T + t) * 8 + e : static_cast<int64_t>(v * 8 + e) * T + t;
-}
-
-template <int T, bool VEC, bool BF16>
-__device__ __forceinline__ Raw load_piece(const void* row, int t, int v, int64_t cols) {
-    Raw r;
-    if constexpr (VEC) {
-        const int64_t c = column<T, true>(t, v, 0);
-        if (c < cols) {
-            if constexpr (BF16) {
-                const uint4 q = *reinterpret_cast<const uint4*>(static_cast<const uint16_t*>(row) + c);
-                r.w[0] = q.x; r.w[1] = q.y; r.w[2] = q.z; r.w[3] = q.w;
-            } else {
-                const uint4* src = reinterpret_cast<const uint4*>(static_cast<const float*>(row) + c);
-                const uint4 a = src[0], b = src[1];
-                r.w[0] = a.x; r.w[1] = a.y; r.w[2] = a.z; r.w[3] = a.w;
-                r.w[4] = b.x; r.w[5] = b.y; r.w[6] = b.z; r.w[7] = b.w;
-            }
-        } else {
-#pragma unroll
-            for (int e = 0; e < (BF16 ? 4 : 8); ++e) r.w[e] = 0;
-        }
-    } else {
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int64_t c = column<T, false>(t, v, e);
-            if (BF16) r.w[e] = c < cols ? static_cast<uint32_t>(static_cast<const uint16_t*>(row)[c]) << 16 : 0;
-            else r.w[e] = c < cols ? static_cast<const uint32_t*>(row)[c] : 0;
-        }
-    }
-    return r;
-}
-
-template <bool VEC, bool BF16>
-__device__ __forceinline__ float value(const Raw& r, int e) {
-    if constexpr (VEC && BF16)
-        return __uint_as_float(e & 1 ? r.w[e >> 1] & 0xFFFF0000u : r.w[e >> 1] << 16);
+// Copies from global to shared memory that run on while their thread computes. A thread waits for its own copies only;
+// what other threads copied it sees after a barrier.
+template <int BYTES>
+__device__ __forceinline__ void copy_async(uint32_t dst, const void* src) {
+    if constexpr (BYTES == 16)
+        asm volatile("cp.async.cg.shared.global [%0], [%1], 16;" ::"r"(dst), "l"(src) : "memory");
     else
-        return __uint_as_float(r.w[e]);
+        asm volatile("cp.async.ca.shared.global [%0], [%1], 8;" ::"r"(dst), "l"(src) : "memory");
 }
+__device__ __forceinline__ void copies_commit() { asm volatile("cp.async.commit_group;" ::: "memory"); }
+template <int LEFT>
+__device__ __forceinline__ void copies_wait() { asm volatile("cp.async.wait_group %0;" ::"n"(LEFT) : "memory"); }
+
+// The next kernel of the stream may be scheduled from here on / waits here for this one (programmatic launch).
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+
+__device__ __forceinline__ float bf16_value(uint32_t h) { return __uint_as_float(h << 16); }
 
 __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     uint32_t r;
@@ -79,35 +49,173 @@ __device__ __forceinline__ uint32_t bf16_pair(float lo, float hi) {
     return r;
 }
 
-template <int T, bool VEC>
-__device__ __forceinline__ void store_piece(void* row, bool bf16, int t, int v, int64_t cols, const float (&y)[8]) {
-    if constexpr (VEC) {
-        const int64_t c = column<T, true>(t, v, 0);
-        if (c >= cols) return;
-        if (bf16) {
-            *reinterpret_cast<uint4*>(static_cast<uint16_t*>(row) + c) = make_uint4(
-                bf16_pair(y[0], y[1]), bf16_pair(y[2], y[3]), bf16_pair(y[4], y[5]), bf16_pair(y[6], y[7]));
-        } else {
-            float4* dst = reinterpret_cast<float4*>(static_cast<float*>(row) + c);
-            dst[0] = make_float4(y[0], y[1], y[2], y[3]);
-            dst[1] = make_float4(y[4], y[5], y[6], y[7]);
+// Which columns a thread has. G = 8 or 4: groups of G consecutive ones, 16 bytes of the widest type of the call, so that
+// every access of a warp is contiguous; G = 1: single ones, for rows that start anywhere.
+template <int T, int G>
+__device__ __forceinline__ int column(int t, int e) {
+    return (e / G * T + t) * G + e % G;
+}
+
+// Elements are kept in pairs (2k, 2k + 1) for the packed f32x2 arithmetic, which halves the instructions that would
+// otherwise bind these kernels before memory does.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+__device__ __forceinline__ float2 minus(float2 a, float b) { return __fadd2_rn(a, both(-b)); }
+
+__device__ __forceinline__ const uint8_t* row_of(const void* base, int64_t row, int64_t stride, bool bf16) {
+    return static_cast<const uint8_t*>(base) + row * stride * (bf16 ? 2 : 4);
+}
+__device__ __forceinline__ uint8_t* row_of(void* base, int64_t row, int64_t stride, bool bf16) {
+    return static_cast<uint8_t*>(base) + row * stride * (bf16 ? 2 : 4);
+}
+
+// Bytes of a row in shared memory. G = 1 has room for every element of its threads, so that reading one needs no test for
+// the row's end, and keeps the row's position within 16 bytes, hence 16 bytes more.
+__host__ __device__ constexpr int64_t slot_bytes(int64_t elements, bool bf16, bool groups) {
+    return elements * (bf16 ? 2 : 4) + (groups ? 0 : 16);
+}
+
+// Where a row starts within 16 bytes, in global and in shared memory.
+__device__ __forceinline__ int phase_of(const uint8_t* row) { return static_cast<int>(reinterpret_cast<uintptr_t>(row) & 15); }
+
+// The T threads that share a row copy it to `slot`. Groups: each thread its own, which it alone will read. Singles: the
+// 16-byte pieces that lie in the row, one after the other; the up to 15 bytes before and after them go through a register
+// of the first threads (`edge`, put in place by place_edge) so that nothing outside the row is read.
+template <int T, int NE, int G, bool BF16>
+__device__ __forceinline__ void request_row(const uint8_t* row, uint8_t* to, int t, int cols, uint32_t& edge) {
+    constexpr int ES = BF16 ? 2 : 4;
+    const uint32_t slot = static_cast<uint32_t>(__cvta_generic_to_shared(to));
+    if constexpr (G > 1) {
+#pragma unroll
+        for (int e = 0; e < NE; e += G) {
+            const int c = column<T, G>(t, e);
+            if (c < cols) copy_async<G * ES == 8 ? 8 : 16>(slot + c * ES, row + c * ES);
+            if (G * ES == 32 && c < cols) copy_async<16>(slot + c * ES + 16, row + c * ES + 16);
         }
     } else {
+        const int phase = phase_of(row);
+        const int bytes = cols * ES;
+        const int head = min((16 - phase) & 15, bytes);
+        const int pieces = (bytes - head) / 16;
 #pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const int64_t c = column<T, false>(t, v, e);
-            if (c >= cols) continue;
-            if (bf16) static_cast<uint16_t*>(row)[c] = static_cast<uint16_t>(bf16_pair(y[e], 0.0f));
-            else static_cast<float*>(row)[c] = y[e];
+        for (int i = 0; i < (NE * ES + 15) / 16; ++i) {
+            const int k = t + i * T;
+            if (k < pieces) copy_async<16>(slot + phase + head + 16 * k, row + head + 16 * k);
+        }
+        // Element t of the edges: `head` bytes in front, then what follows the pieces.
+        if (t * ES < 32) {
+            const int at = t * ES < head ? t * ES : t * ES + 16 * pieces;
+            if (at < bytes)
+                edge = BF16 ? *reinterpret_cast<const uint16_t*>(row + at) : *reinterpret_cast<const uint32_t*>(row + at);
         }
     }
 }
 
-template <int T, bool VEC>
-__device__ __forceinline__ void load_params(const float* p, int t, int v, int64_t cols, float (&out)[8]) {
-    const Raw r = load_piece<T, VEC, false>(p, t, v, cols);
+// Also clears what is read of the 16 bytes past the row's end, which hold what an earlier row at another position left.
+template <int ELEMENTS, bool BF16>
+__device__ __forceinline__ void place_edge(int phase, uint8_t* slot, int t, int cols, uint32_t edge) {
+    constexpr int ES = BF16 ? 2 : 4;
+    if (t * ES >= 48) return;
+    const int bytes = cols * ES;
+    const int head = min((16 - phase) & 15, bytes);
+    const int at = t * ES < head ? t * ES : t * ES + (bytes - head) / 16 * 16;
+    if (at >= min(bytes + 16, ELEMENTS * ES)) return;
+    const uint32_t v = at < bytes ? edge : 0;
+    if (BF16) *reinterpret_cast<uint16_t*>(slot + phase + at) = static_cast<uint16_t>(v);
+    else *reinterpret_cast<uint32_t*>(slot + phase + at) = v;
+}
+
+// Fills a ring with zeros, which is what stays past the rows' ends.
+__device__ __forceinline__ void clear(uint8_t* ring, int bytes) {
+    for (int i = threadIdx.x * 16; i < bytes; i += blockDim.x * 16) *reinterpret_cast<uint4*>(ring + i) = make_uint4(0, 0, 0, 0);
+    __syncthreads();
+}
+
+// A thread's elements of a row from shared memory. (Groups: volatile reads, each behind its test, so that the compiler
+// does not move all of them up and spill what they would hold: 94 us against 55 us for the backward pass of 65,536 x 768.)
+template <int T, int NE, int G, bool BF16>
+__device__ __forceinline__ void read_row(int phase, const uint8_t* slot, int t, int cols, float2 (&v)[NE / 2]) {
+    constexpr int ES = BF16 ? 2 : 4;
+    if constexpr (G > 1) {
+        constexpr int PER = G * ES == 8 ? 4 : 16 / ES;  // elements of one access
+        const uint32_t mine = static_cast<uint32_t>(__cvta_generic_to_shared(slot)) + t * G * ES;
 #pragma unroll
-    for (int e = 0; e < 8; ++e) out[e] = __uint_as_float(r.w[e]);
+        for (int e = 0; e < NE; e += PER) {
+            const uint32_t at = mine + (e / G * T * G + e % G) * ES;
+            uint32_t w[4] = {0, 0, 0, 0};
+            if (column<T, G>(t, e) < cols) {
+                if constexpr (G * ES == 8)
+                    asm volatile("ld.shared.v2.u32 {%0, %1}, [%2];" : "=r"(w[0]), "=r"(w[1]) : "r"(at));
+                else
+                    asm volatile("ld.shared.v4.u32 {%0, %1, %2, %3}, [%4];"
+                                 : "=r"(w[0]), "=r"(w[1]), "=r"(w[2]), "=r"(w[3]) : "r"(at));
+            }
+#pragma unroll
+            for (int k = 0; k < PER / 2; ++k)
+                v[e / 2 + k] = BF16 ? make_float2(__uint_as_float(w[k] << 16), __uint_as_float(w[k] & 0xFFFF0000u))
+                                    : make_float2(__uint_as_float(w[(2 * k) & 3]), __uint_as_float(w[(2 * k + 1) & 3]));
+        }
+    } else {
+        const uint8_t* mine = slot + phase + t * ES;
+        float one[NE];
+#pragma unroll
+        for (int e = 0; e < NE; ++e)
+            one[e] = BF16 ? bf16_value(*reinterpret_cast<const uint16_t*>(mine + e * T * ES))
+                          : *reinterpret_cast<const float*>(mine + e * T * ES);
+#pragma unroll
+        for (int k = 0; k < NE / 2; ++k) v[k] = make_float2(one[2 * k], one[2 * k + 1]);
+    }
+}
+
+template <int T, int NE, int G>
+__device__ __forceinline__ void load_params(const float* p, int t, int cols, float2 (&v)[NE / 2]) {
+#pragma unroll
+    for (int e = 0; e < NE; e += G == 1 ? 2 : 4) {
+        const int c = column<T, G>(t, e);
+        if constexpr (G == 1) {
+            const int next = column<T, 1>(t, e + 1);
+            v[e / 2] = make_float2(c < cols ? __ldg(p + c) : 0.0f, next < cols ? __ldg(p + next) : 0.0f);
+        } else {
+            const float4 q = c < cols ? __ldg(reinterpret_cast<const float4*>(p + c)) : make_float4(0, 0, 0, 0);
+            v[e / 2] = make_float2(q.x, q.y);
+            v[e / 2 + 1] = make_float2(q.z, q.w);
+        }
+    }
+}
+
+template <int T, int NE, int G>
+__device__ __forceinline__ void store_row(uint8_t* row, bool bf16, int t, int cols, const float2 (&y)[NE / 2]) {
+    if constexpr (G == 1) {
+        const int left = cols - t;
+        if (bf16) {
+            uint16_t* mine = reinterpret_cast<uint16_t*>(row) + t;
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+                if (e * T < left) mine[e * T] = static_cast<uint16_t>(bf16_pair(e & 1 ? y[e / 2].y : y[e / 2].x, 0.0f));
+        } else {
+            float* mine = reinterpret_cast<float*>(row) + t;
+#pragma unroll
+            for (int e = 0; e < NE; ++e)
+                if (e * T < left) mine[e * T] = e & 1 ? y[e / 2].y : y[e / 2].x;
+        }
+    } else {
+#pragma unroll
+        for (int e = 0; e < NE; e += G) {
+            const int c = column<T, G>(t, e);
+            if (c >= cols) continue;
+            const float2* q = y + e / 2;
+            if (!bf16) {
+#pragma unroll
+                for (int k = 0; k < G; k += 4)
+                    *reinterpret_cast<float4*>(row + (c + k) * 4) =
+                        make_float4(q[k / 2].x, q[k / 2].y, q[k / 2 + 1].x, q[k / 2 + 1].y);
+            } else if constexpr (G == 8) {
+                *reinterpret_cast<uint4*>(row + c * 2) = make_uint4(bf16_pair(q[0].x, q[0].y), bf16_pair(q[1].x, q[1].y),
+                                                                    bf16_pair(q[2].x, q[2].y), bf16_pair(q[3].x, q[3].y));
+            } else {
+                *reinterpret_cast<uint2*>(row + c * 2) = make_uint2(bf16_pair(q[0].x, q[0].y), bf16_pair(q[1].x, q[1].y));
+            }
+        }
+    }
 }
 
 __device__ __forceinline__ float2 warp_sum2(float2 v) {
@@ -136,11 +244,23 @@ __device__ __forceinline__ float2 row_sum2(float2 v, float2 (*part)[32], int& tu
     return v;
 }
 
-__device__ __forceinline__ const void* row_of(const void* base, int64_t row, int64_t stride, bool bf16) {
-    return static_cast<const uint8_t*>(base) + row * stride * (bf16 ? 2 : 4);
+// The same of one value in both halves (their sum over the threads).
+template <int T>
+__device__ __forceinline__ float row_sum(float2 v, float2 (*part)[32], int& turn) {
+    float one = v.x + v.y;
+    if constexpr (T == 32) {
+#pragma unroll
+        for (int s = 16; s > 0; s >>= 1) one += __shfl_xor_sync(0xffffffffu, one, s);
+        return one;
+    } else {
+        return row_sum2<T>(make_float2(one, 0.0f), part, turn).x;
+    }
 }
-__device__ __forceinline__ void* row_of(void* base, int64_t row, int64_t stride, bool bf16) {
-    return static_cast<uint8_t*>(base) + row * stride * (bf16 ? 2 : 4);
+
+template <int T>
+__device__ __forceinline__ void row_barrier() {
+    if constexpr (T == 32) __syncwarp();
+    else __syncthreads();
 }
 
 struct NormParams {
@@ -156,153 +276,261 @@ struct NormParams {
     float* mean;
     float* inv_std;
     float* sums;        // backward: [2, grid, cols] partial dg and db
+    int32_t depth;      // rows in flight
 };
 
-// T threads a row, NV pieces of 8 elements a thread.
-template <int T, int NV, bool VEC, bool XB>
-__global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T) layer_norm_kernel(const NormParams p) {
+// Both kernels: T threads a row, NE elements a thread, `depth` rows in flight in shared memory (a ring for each warp when
+// T is 32, else one of the block), rows first, first + step, ... . kMaxDepth bounds the waits' immediate operands.
+constexpr int kMaxDepth = 4;
+
+__device__ __forceinline__ void wait_for_row(int depth) {
+    // All but the newest depth - 1 groups of copies have arrived.
+    if (depth >= 4) copies_wait<3>();
+    else if (depth == 3) copies_wait<2>();
+    else if (depth == 2) copies_wait<1>();
+    else copies_wait<0>();
+}
+
+template <int T, int NE, int G, bool XB>
+__global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T == 32 ? 2 : 1) layer_norm_kernel(const NormParams p) {
+    extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 part[2][32];
     int turn = 0;
     const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t row = T == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5) : blockIdx.x;
-    if (row >= p.rows) return;
-    const void* x = row_of(p.x, row, p.x_stride, XB);
-    Raw r[NV];
-#pragma unroll
-    for (int v = 0; v < NV; ++v) r[v] = load_piece<T, VEC, XB>(x, t, v, p.cols);
-    float sum = 0.0f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) sum += value<VEC, XB>(r[v], e);
-    const float mean = row_sum2<T>(make_float2(sum, 0.0f), part, turn).x / static_cast<float>(p.cols);
-    float squares = 0.0f;
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) {
-            const float d = value<VEC, XB>(r[v], e) - mean;
-            squares += column<T, VEC>(t, v, e) < p.cols ? d * d : 0.0f;
+    const int warp = threadIdx.x >> 5;
+    const int64_t first = T == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + warp : blockIdx.x;
+    const int64_t step = T == 32 ? static_cast<int64_t>(gridDim.x) * kWarpsPerBlock : gridDim.x;
+    const int cols = static_cast<int>(p.cols);
+    constexpr int slot = static_cast<int>(slot_bytes(T * NE, XB, G > 1));
+    if constexpr (G == 1) clear(ring, slot * p.depth * (T == 32 ? kWarpsPerBlock : 1));
+    uint8_t* base = ring + (T == 32 ? warp * p.depth * slot : 0);
+    uint32_t edge = 0;
+    int phase = 0;  // of the row asked for last
+    int64_t ahead = first;
+    const int64_t x_step = step * p.x_stride * (XB ? 2 : 4), y_step = step * p.y_stride * (p.y_bf16 ? 2 : 4);
+    const uint8_t* x = row_of(p.x, first, p.x_stride, XB);
+    uint8_t* y = row_of(p.y, first, p.y_stride, p.y_bf16);
+    int in = 0, out = 0;
+    auto request = [&]() {
+        if (ahead < p.rows) {
+            request_row<T, NE, G, XB>(x, base + in * slot, t, cols, edge);
+            if (G == 1) phase = phase_of(x);
         }
-    const float variance = row_sum2<T>(make_float2(squares, 0.0f), part, turn).x / static_cast<float>(p.cols);
-    const float inv = 1.0f / sqrtf(variance + p.epsilon);
-    if (t == 0) {
-        p.mean[row] = mean;
-        p.inv_std[row] = inv;
+        copies_commit();
+        ahead += step;
+        x += x_step;
+        if (++in == p.depth) in = 0;
+    };
+    // Singles' edges pass through one register: their rows are requested one ahead only.
+    for (int k = 0; k < (G > 1 ? p.depth - 1 : 1); ++k) request();
+    float2 gain[NE / 2], bias[NE / 2];
+    load_params<T, NE, G>(p.gain, t, cols, gain);
+    if (p.bias != nullptr) {
+        load_params<T, NE, G>(p.bias, t, cols, bias);
+    } else {
+#pragma unroll
+        for (int k = 0; k < NE / 2; ++k) bias[k] = both(0.0f);
     }
-    void* y = row_of(p.y, row, p.y_stride, p.y_bf16);
-#pragma unroll
-    for (int v = 0; v < NV; ++v) {
-        float g[8], b[8], out[8];
-        load_params<T, VEC>(p.gain, t, v, p.cols, g);
-        if (p.bias != nullptr) {
-            load_params<T, VEC>(p.bias, t, v, p.cols, b);
+    const float columns = static_cast<float>(cols);
+    for (int64_t row = first; row < p.rows; row += step) {
+        const int here = phase;
+        if constexpr (G > 1) {
+            request();
+            wait_for_row(p.depth);
         } else {
+            copies_wait<0>();
+            place_edge<T * NE, XB>(here, base + out * slot, t, cols, edge);
+            row_barrier<T>();
+            request();
+        }
+        float2 v[NE / 2];
+        read_row<T, NE, G, XB>(here, base + out * slot, t, cols, v);
+        if (++out == p.depth) out = 0;
+        float2 sum = both(0.0f);
 #pragma unroll
-            for (int e = 0; e < 8; ++e) b[e] = 0.0f;
+        for (int k = 0; k < NE / 2; ++k) sum = __fadd2_rn(sum, v[k]);
+        const float mean = row_sum<T>(sum, part, turn) / columns;
+        float2 squares = both(0.0f);
+#pragma unroll
+        for (int k = 0; k < NE / 2; ++k) {
+            v[k] = minus(v[k], mean);
+            // (Groups lie in the row or past it as a whole; singles each by themselves.)
+            const bool in_row = column<T, G>(t, 2 * k) < cols;
+            const bool next_in_row = G > 1 ? in_row : column<T, G>(t, 2 * k + 1) < cols;
+            const float2 live = make_float2(in_row ? v[k].x : 0.0f, next_in_row ? v[k].y : 0.0f);
+            squares = __ffma2_rn(live, live, squares);
+        }
+        const float variance = row_sum<T>(squares, part, turn) / columns;
+        const float inv = 1.0f / sqrtf(variance + p.epsilon);
+        if (t == 0) {
+            p.mean[row] = mean;
+            p.inv_std[row] = inv;
         }
 #pragma unroll
-        for (int e = 0; e < 8; ++e) out[e] = fmaf((value<VEC, XB>(r[v], e) - mean) * inv, g[e], b[e]);
-        store_piece<T, VEC>(y, p.y_bf16, t, v, p.cols, out);
+        for (int k = 0; k < NE / 2; ++k) v[k] = __ffma2_rn(__fmul2_rn(v[k], both(inv)), gain[k], bias[k]);
+        store_row<T, NE, G>(y, p.y_bf16, t, cols, v);
+        y += y_step;
     }
 }
 
-// The backward pass on a fixed grid (see the top): block b's rows, or warps', are b, b + grid, ... . Elements past the
-// row's end are zeros in x and dy, so they add nothing to any sum.
-template <int T, int NV, bool VEC, bool XB, bool DB>
-__global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T == 32 ? 2 : 1)
+// Elements past the row's end are zeros in dy and the gain, so they add nothing to any sum.
+template <int T, int NE, int G, bool XB, bool DB>
+__global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T <= 256 ? 2 : 1)
     layer_norm_backward_kernel(const NormParams p) {
-    extern __shared__ float column_sums[];  // T == 32: [2, cols], the block's sums
+    extern __shared__ __align__(16) uint8_t ring[];
     __shared__ float2 part[2][32];
+    allow_next_kernel();
     int turn = 0;
     const int t = T == 32 ? threadIdx.x & 31 : threadIdx.x;
-    const int64_t first = T == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + (threadIdx.x >> 5) : blockIdx.x;
+    const int warp = threadIdx.x >> 5;
+    const int64_t first = T == 32 ? static_cast<int64_t>(blockIdx.x) * kWarpsPerBlock + warp : blockIdx.x;
     const int64_t step = T == 32 ? static_cast<int64_t>(gridDim.x) * kWarpsPerBlock : gridDim.x;
-    const float per_column = 1.0f / static_cast<float>(p.cols);
-    float dg[NV][8], db[NV][8];
-#pragma unroll
-    for (int v = 0; v < NV; ++v)
-#pragma unroll
-        for (int e = 0; e < 8; ++e) dg[v][e] = db[v][e] = 0.0f;
-    Raw x[NV], dy[NV];
-    float mean = 0.0f, inv = 0.0f;
-    auto request = [&](int64_t row) {
-        const void* xr = row_of(p.x, row, p.x_stride, XB);
-        const void* dr = row_of(p.dy, row, p.dy_stride, DB);
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            x[v] = load_piece<T, VEC, XB>(xr, t, v, p.cols);
-            dy[v] = load_piece<T, VEC, DB>(dr, t, v, p.cols);
+    const int cols = static_cast<int>(p.cols);
+    constexpr int x_slot = static_cast<int>(slot_bytes(T * NE, XB, G > 1));
+    constexpr int slot = x_slot + static_cast<int>(slot_bytes(T * NE, DB, G > 1));
+    if constexpr (G == 1) clear(ring, slot * p.depth * (T == 32 ? kWarpsPerBlock : 1));
+    uint8_t* base = ring + (T == 32 ? warp * p.depth * slot : 0);
+    uint32_t x_edge = 0, dy_edge = 0;
+    int x_phase = 0, dy_phase = 0;              // of the row asked for last
+    float mean_ahead = 0.0f, inv_ahead = 0.0f;  // of the next row
+    int64_t ahead = first;
+    const int64_t x_step = step * p.x_stride * (XB ? 2 : 4), dy_step = step * p.dy_stride * (DB ? 2 : 4);
+    const int64_t dx_step = step * p.y_stride * (XB ? 2 : 4);
+    const uint8_t* x = row_of(p.x, first, p.x_stride, XB);
+    const uint8_t* dy = row_of(p.dy, first, p.dy_stride, DB);
+    uint8_t* dx = row_of(p.y, first, p.y_stride, XB);
+    int in = 0, out = 0;
+    auto request = [&]() {
+        if (ahead < p.rows) {
+            request_row<T, NE, G, XB>(x, base + in * slot, t, cols, x_edge);
+            request_row<T, NE, G, DB>(dy, base + in * slot + x_slot, t, cols, dy_edge);
+            if (G == 1) {
+                x_phase = phase_of(x);
+                dy_phase = phase_of(dy);
+            }
         }
-        mean = __ldg(p.mean + row);
-        inv = __ldg(p.inv_std + row);
+        copies_commit();
+        ahead += step;
+        x += x_step;
+        dy += dy_step;
+        if (++in == p.depth) in = 0;
     };
+    auto statistics = [&](int64_t row) {
+        if (row < p.rows) {
+            mean_ahead = __ldg(p.mean + row);
+            inv_ahead = __ldg(p.inv_std + row);
+        }
+    };
+    for (int k = 0; k < (G > 1 ? p.depth - 1 : 1); ++k) request();
+    statistics(first);
+    // With 24 elements a thread the gain's registers would be the ones too many: a warp's share a copy, in the order in
+    // which the threads read it.
+    constexpr bool kSharedGain = NE >= 24;
+    __shared__ float4 shared_gain[kSharedGain ? NE / 4 : 1][T];
+    float2 gain[NE / 2], dg[NE / 2], db[NE / 2];
+    if constexpr (kSharedGain) {
+        load_params<T, NE, G>(p.gain, t, cols, gain);
+        if (T > 32 || warp == 0) {
+#pragma unroll
+            for (int k = 0; k < NE / 4; ++k)
+                shared_gain[k][t] = make_float4(gain[2 * k].x, gain[2 * k].y, gain[2 * k + 1].x, gain[2 * k + 1].y);
+        }
+        __syncthreads();
+    } else {
+        load_params<T, NE, G>(p.gain, t, cols, gain);
+    }
+#pragma unroll
+    for (int k = 0; k < NE / 2; ++k) dg[k] = db[k] = both(0.0f);
+    const float per_column = 1.0f / static_cast<float>(cols);
     for (int64_t row = first; row < p.rows; row += step) {
-        request(row);
-        float2 s = make_float2(0.0f, 0.0f);
-#pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float g[8];
-            load_params<T, VEC>(p.gain, t, v, p.cols, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float n = (value<VEC, XB>(x[v], e) - mean) * inv;
-                const float o = value<VEC, DB>(dy[v], e);
-                s.x += o * g[e];
-                s.y += o * g[e] * n;
-                db[v][e] += o;
-                dg[v][e] += o * n;
-            }
+        const int x_here = x_phase, dy_here = dy_phase;
+        uint8_t* here = base + out * slot;
+        const float mean = mean_ahead, inv = inv_ahead;
+        if constexpr (G > 1) {
+            request();
+            statistics(row + step);
+            wait_for_row(p.depth);
+        } else {
+            // (A slot is asked for again two rows later at the earliest, behind the barrier of the row in between.)
+            copies_wait<0>();
+            place_edge<T * NE, XB>(x_here, here, t, cols, x_edge);
+            place_edge<T * NE, DB>(dy_here, here + x_slot, t, cols, dy_edge);
+            row_barrier<T>();
+            request();
+            statistics(row + step);
         }
-        s = row_sum2<T>(s, part, turn);
+        if (++out == p.depth) out = 0;
+        // d = dy g of one pair of elements.
+        auto gained = [&](float2 o, int k) {
+            if constexpr (kSharedGain) {
+                const float4 g = shared_gain[k / 2][t];
+                return __fmul2_rn(o, k & 1 ? make_float2(g.z, g.w) : make_float2(g.x, g.y));
+            } else {
+                return __fmul2_rn(o, gain[k]);
+            }
+        };
+        float2 sum = both(0.0f), product = both(0.0f);
+        float2 n[NE / 2], d[NE / 2];
+        read_row<T, NE, G, XB>(x_here, here, t, cols, n);
+        read_row<T, NE, G, DB>(dy_here, here + x_slot, t, cols, d);
+#pragma unroll
+        for (int k = 0; k < NE / 2; ++k) {
+            n[k] = __fmul2_rn(minus(n[k], mean), both(inv));
+            db[k] = __fadd2_rn(db[k], d[k]);
+            dg[k] = __ffma2_rn(d[k], n[k], dg[k]);
+            d[k] = gained(d[k], k);
+            sum = __fadd2_rn(sum, d[k]);
+            product = __ffma2_rn(d[k], n[k], product);
+        }
+        const float2 s = row_sum2<T>(make_float2(sum.x + sum.y, product.x + product.y), part, turn);
         const float mean_d = s.x * per_column, mean_dn = s.y * per_column;
-        void* out = row_of(p.y, row, p.y_stride, XB);
+        if constexpr (kSharedGain) {
+            // Held until here the row would not fit beside the column sums: it is read from shared memory again.
+            read_row<T, NE, G, XB>(x_here, here, t, cols, n);
+            read_row<T, NE, G, DB>(dy_here, here + x_slot, t, cols, d);
 #pragma unroll
-        for (int v = 0; v < NV; ++v) {
-            float g[8], dx[8];
-            load_params<T, VEC>(p.gain, t, v, p.cols, g);
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const float n = (value<VEC, XB>(x[v], e) - mean) * inv;
-                dx[e] = inv * (value<VEC, DB>(dy[v], e) * g[e] - mean_d - n * mean_dn);
+            for (int k = 0; k < NE / 2; ++k) {
+                n[k] = __fmul2_rn(minus(n[k], mean), both(inv));
+                d[k] = gained(d[k], k);
             }
-            store_piece<T, VEC>(out, XB, t, v, p.cols, dx);
         }
+#pragma unroll
+        for (int k = 0; k < NE / 2; ++k)
+            d[k] = __fmul2_rn(both(inv), __ffma2_rn(n[k], both(-mean_dn), minus(d[k], mean_d)));
+        store_row<T, NE, G>(dx, XB, t, cols, d);
+        dx += dx_step;
     }
     float* out_g = p.sums + static_cast<int64_t>(blockIdx.x) * p.cols;
     float* out_b = out_g + static_cast<int64_t>(gridDim.x) * p.cols;
     if constexpr (T == 32) {
-        // The block's warps add their sums one after the other.
-        for (int w = 0; w < kWarpsPerBlock; ++w) {
-            if (static_cast<int>(threadIdx.x >> 5) == w) {
+        // The block's warps leave their sums in the ring's memory, where they are added up in warp order.
+        copies_wait<0>();
+        __syncthreads();
+        float* sums = reinterpret_cast<float*>(ring);
 #pragma unroll
-                for (int v = 0; v < NV; ++v)
-#pragma unroll
-                    for (int e = 0; e < 8; ++e) {
-                        const int64_t c = column<T, VEC>(t, v, e);
-                        if (c < p.cols) {
-                            column_sums[c] = (w > 0 ? column_sums[c] : 0.0f) + dg[v][e];
-                            column_sums[p.cols + c] = (w > 0 ? column_sums[p.cols + c] : 0.0f) + db[v][e];
-                        }
-                    }
+        for (int e = 0; e < NE; ++e) {
+            const int c = column<T, G>(t, e);
+            if (c < cols) {
+                sums[(2 * warp) * cols + c] = e & 1 ? dg[e / 2].y : dg[e / 2].x;
+                sums[(2 * warp + 1) * cols + c] = e & 1 ? db[e / 2].y : db[e / 2].x;
             }
-            __syncthreads();
         }
-        for (int64_t c = threadIdx.x; c < p.cols; c += blockDim.x) {
-            out_g[c] = column_sums[c];
-            out_b[c] = column_sums[p.cols + c];
+        __syncthreads();
+        for (int c = threadIdx.x; c < 2 * cols; c += blockDim.x) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int w = 0; w < kWarpsPerBlock; ++w) sum += sums[2 * w * cols + c];
+            (c < cols ? out_g + c : out_b + c - cols)[0] = sum;
         }
     } else {
 #pragma unroll
-        for (int v = 0; v < NV; ++v)
-#pragma unroll
-            for (int e = 0; e < 8; ++e) {
-                const int64_t c = column<T, VEC>(t, v, e);
-                if (c < p.cols) {
-                    out_g[c] = dg[v][e];
-                    out_b[c] = db[v][e];
-                }
+        for (int e = 0; e < NE; ++e) {
+            const int c = column<T, G>(t, e);
+            if (c < cols) {
+                out_g[c] = e & 1 ? dg[e / 2].y : dg[e / 2].x;
+                out_b[c] = e & 1 ? db[e / 2].y : db[e / 2].x;
             }
+        }
     }
 }
 
@@ -314,6 +542,7 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* s
     const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
     const int64_t c = static_cast<int64_t>(blockIdx.x) * 32 + lane;
     float* out = blockIdx.y == 0 ? gain_grad : bias_grad;
+    wait_for_previous_kernel();
     if (out == nullptr) return;
     const float* src = sums + static_cast<int64_t>(blockIdx.y) * parts * cols;
     float s = 0.0f;
@@ -404,22 +633,34 @@ __global__ void __launch_bounds__(256) layer_norm_wide_columns_kernel(const Norm
     p.sums[static_cast<int64_t>(gridDim.y + blockIdx.y) * p.cols + c] = db;
 }
 
-// How a row is held: T threads with NV pieces of 8 elements. T = 0: not at all (the wide kernels). A warp alone needs no
-// barrier, but past 1,024 columns its registers run out; blocks are as narrow as holds the row in few pieces, since
-// barriers cost more the more warps meet.
+// How a row is held: T threads with up to `elements` each. T = 0: not at all (the wide kernels). A warp alone needs no
+// barrier, but past 1,024 columns (768 in the backward pass, which holds five values for each) its registers run out.
+// Blocks are as narrow as can hold the row: what binds them is the chain of barriers and reads of a row, so two blocks of
+// 256 threads on an SM, with a row each, beat one of 512 (backward pass of 3,001 x 5,003 bf16: 30 us, with 512 threads
+// 46 us, with 1,024 50 us).
 struct Shape {
-    int threads, pieces;
+    int threads, elements;
 };
 
 Shape shape_of(uint64_t cols, bool backward) {
-    if (cols <= 1024) return {32, static_cast<int>((cols + 255) / 256)};
-    if (cols <= 2048) return {256, 1};
-    if (cols <= 4096) return {512, 1};
-    if (cols <= 8192) return {512, 2};
-    // The backward pass holds four values for each column of a thread's.
-    if (!backward && cols <= 16384) return {1024, 2};
-    if (!backward && cols <= 32768) return {1024, 4};
+    if (cols <= (backward ? 768 : 1024)) return {32, static_cast<int>((cols + 255) / 256) * 8};
+    if (cols <= 1024) return {128, 8};
+    if (cols <= 2048) return {256, 8};
+    if (backward && cols <= 6144) return {256, cols <= 4096 ? 16 : cols <= 5120 ? 20 : 24};
+    if (cols <= 4096) return {512, 8};
+    if (cols <= 6144) return {512, 12};
+    if (cols <= 8192) return {512, 16};
+    if (!backward && cols <= 16384) return {1024, 16};
     return {0, 0};
+}
+
+constexpr int64_t kRingBytes = 96 << 10;  // of a wide thread block, so that two fit on an SM
+
+// Rows in flight: as many as kMaxDepth and the ring allow, at least two.
+int depth_of(const Shape& s, int64_t row_bytes) {
+    const int64_t rings = s.threads == 32 ? kWarpsPerBlock : 1;
+    const int64_t bytes = s.threads == 128 ? kRingBytes / 3 : kRingBytes - (24 << 10);  // (a gain's copy takes 24 KB)
+    return static_cast<int>(std::max<int64_t>(2, std::min<int64_t>(kMaxDepth, bytes / (rings * row_bytes))));
 }
 
 // Blocks of the backward pass, which is also how many partial sums there are.
@@ -427,7 +668,7 @@ uint64_t backward_grid(uint64_t rows, uint64_t cols, int sms) {
     const Shape s = shape_of(cols, true);
     if (s.threads == 0) return std::min<uint64_t>(rows, 64);
     if (s.threads == 32) return std::min<uint64_t>((rows + kWarpsPerBlock - 1) / kWarpsPerBlock, 2ull * sms);
-    return std::min<uint64_t>(rows, (s.threads == 256 ? 3ull : s.pieces == 1 ? 2ull : 1ull) * sms);
+    return std::min<uint64_t>(rows, (s.threads == 128 ? 4ull : s.threads == 256 ? 2ull : 1ull) * sms);
 }
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -439,34 +680,57 @@ int launched(const char* what, std::string* err) {
     return SNB_ERR_CUDA;
 }
 
-template <int T, int NV, bool VEC>
-void forward_typed(const NormParams& p, unsigned grid, cudaStream_t s) {
-    const int threads = T == 32 ? 32 * kWarpsPerBlock : T;
-    if (p.x_bf16) layer_norm_kernel<T, NV, VEC, true><<<grid, threads, 0, s>>>(p);
-    else layer_norm_kernel<T, NV, VEC, false><<<grid, threads, 0, s>>>(p);
+// Launches `kernel` with a ring of its own size. Above 48 KB together with the kernel's static shared memory (4 KB at
+// most) that has to be allowed first, a setting of the kernel on the current device that is cheap to repeat.
+template <typename Kernel>
+void launch_ring(Kernel kernel, unsigned grid, int threads, int64_t smem, cudaStream_t s, const NormParams& p) {
+    if (smem > (44 << 10))
+        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+    kernel<<<grid, threads, static_cast<size_t>(smem), s>>>(p);
 }
 
-template <int T, int NV>
-void forward_shaped(const NormParams& p, bool vec, cudaStream_t s) {
-    const unsigned grid = static_cast<unsigned>(T == 32 ? (p.rows + kWarpsPerBlock - 1) / kWarpsPerBlock : p.rows);
-    if (vec) forward_typed<T, NV, true>(p, grid, s);
-    else forward_typed<T, NV, false>(p, grid, s);
+template <int T, int NE, int G>
+void forward_typed(NormParams p, int sms, cudaStream_t s) {
+    constexpr int threads = T == 32 ? 32 * kWarpsPerBlock : T;
+    const int64_t slot = slot_bytes(T * NE, p.x_bf16 != 0, G > 1);
+    p.depth = depth_of({T, NE}, slot);
+    const int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
+    const int64_t blocks = T == 32 ? (p.rows + kWarpsPerBlock - 1) / kWarpsPerBlock : p.rows;
+    const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, (T == 1024 ? 1ll : T == 256 ? 4ll : 2ll) * sms));
+    if (p.x_bf16) launch_ring(layer_norm_kernel<T, NE, G, true>, grid, threads, smem, s, p);
+    else launch_ring(layer_norm_kernel<T, NE, G, false>, grid, threads, smem, s, p);
 }
 
-template <int T, int NV, bool VEC>
-void backward_typed(const NormParams& p, unsigned grid, cudaStream_t s) {
-    const int threads = T == 32 ? 32 * kWarpsPerBlock : T;
-    const size_t smem = T == 32 ? 2 * p.cols * sizeof(float) : 0;
-    if (p.x_bf16 && p.dy_bf16) layer_norm_backward_kernel<T, NV, VEC, true, true><<<grid, threads, smem, s>>>(p);
-    else if (p.x_bf16) layer_norm_backward_kernel<T, NV, VEC, true, false><<<grid, threads, smem, s>>>(p);
-    else if (p.dy_bf16) layer_norm_backward_kernel<T, NV, VEC, false, true><<<grid, threads, smem, s>>>(p);
-    else layer_norm_backward_kernel<T, NV, VEC, false, false><<<grid, threads, smem, s>>>(p);
+// group: the columns of 16 bytes of the call's widest type, or 1 where its rows do not allow 16-byte accesses.
+template <int T, int NE>
+void forward_shaped(const NormParams& p, int group, int sms, cudaStream_t s) {
+    if (group == 8) forward_typed<T, (NE + 7) / 8 * 8, 8>(p, sms, s);
+    else if (group == 4) forward_typed<T, NE, 4>(p, sms, s);
+    else forward_typed<T, NE, 1>(p, sms, s);
 }
 
-template <int T, int NV>
-void backward_shaped(const NormParams& p, bool vec, unsigned grid, cudaStream_t s) {
-    if (vec) backward_typed<T, NV, true>(p, grid, s);
-    else backward_typed<T, NV, false>(p, grid, s);
+template <int T, int NE, int G>
+void backward_typed(NormParams p, unsigned grid, cudaStream_t s) {
+    constexpr int threads = T == 32 ? 32 * kWarpsPerBlock : T;
+    const int64_t slot = slot_bytes(T * NE, p.x_bf16 != 0, G > 1) + slot_bytes(T * NE, p.dy_bf16 != 0, G > 1);
+    p.depth = depth_of({T, NE}, slot);
+    int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
+    if (T == 32) smem = std::max<int64_t>(smem, 2 * kWarpsPerBlock * p.cols * static_cast<int64_t>(sizeof(float)));
+    if (p.x_bf16 && p.dy_bf16) launch_ring(layer_norm_backward_kernel<T, NE, G, true, true>, grid, threads, smem, s, p);
+    else if (p.x_bf16) {
+        if constexpr (G != 8) launch_ring(layer_norm_backward_kernel<T, NE, G, true, false>, grid, threads, smem, s, p);
+    } else if (p.dy_bf16) {
+        if constexpr (G != 8) launch_ring(layer_norm_backward_kernel<T, NE, G, false, true>, grid, threads, smem, s, p);
+    } else {
+        if constexpr (G != 8) launch_ring(layer_norm_backward_kernel<T, NE, G, false, false>, grid, threads, smem, s, p);
+    }
+}
+
+template <int T, int NE>
+void backward_shaped(const NormParams& p, int group, unsigned grid, cudaStream_t s) {
+    if (group == 8) backward_typed<T, (NE + 7) / 8 * 8, 8>(p, grid, s);
+    else if (group == 4) backward_typed<T, NE, 4>(p, grid, s);
+    else backward_typed<T, NE, 1>(p, grid, s);
 }
 
 NormParams params_of(const snb_layer_norm_args& a) {
@@ -484,9 +748,10 @@ NormParams params_of(const snb_layer_norm_args& a) {
     return p;
 }
 
-// Whether a tensor's rows can be read 8 elements at a time.
-bool vectors(const void* base, uint64_t stride, uint64_t cols, int type) {
-    return aligned16(base) && cols % 8 == 0 && stride * (type == SNB_TYPE_BF16 ? 2 : 4) % 16 == 0;
+// Whether every row of a tensor can be taken in whole 16-byte pieces.
+bool pieces16(const void* base, uint64_t stride, uint64_t cols, int type) {
+    const uint64_t es = type == SNB_TYPE_BF16 ? 2 : 4;
+    return aligned16(base) && cols * es % 16 == 0 && stride * es % 16 == 0;
 }
 
 }  // namespace
@@ -505,19 +770,25 @@ int layer_norm_forward_launch(cudaStream_t s, const snb_layer_norm_args& a, std:
     p.y = a.output;
     p.y_stride = static_cast<int64_t>(a.output_stride);
     p.y_bf16 = a.output_type == SNB_TYPE_BF16;
-    const bool vec = vectors(a.input, a.input_stride, a.cols, a.input_type) &&
-                     vectors(a.output, a.output_stride, a.cols, a.output_type) && aligned16(a.gain) && aligned16(a.bias);
+    DeviceInfo dev;
+    const int rc = current_device_info(&dev, err);
+    if (rc != SNB_OK) return rc;
+    const bool whole = pieces16(a.input, a.input_stride, a.cols, a.input_type) &&
+                       pieces16(a.output, a.output_stride, a.cols, a.output_type) && aligned16(a.gain) &&
+                       aligned16(a.bias);
+    // (An f32 output of a bf16 input keeps groups of 8: two stores of 16 bytes.)
+    const int group = !whole ? 1 : p.x_bf16 ? 8 : 4;
     const Shape shape = shape_of(a.cols, false);
-    switch (shape.threads * 8 + shape.pieces) {
-        case 32 * 8 + 1: forward_shaped<32, 1>(p, vec, s); break;
-        case 32 * 8 + 2: forward_shaped<32, 2>(p, vec, s); break;
-        case 32 * 8 + 3: forward_shaped<32, 3>(p, vec, s); break;
-        case 32 * 8 + 4: forward_shaped<32, 4>(p, vec, s); break;
-        case 256 * 8 + 1: forward_shaped<256, 1>(p, vec, s); break;
-        case 512 * 8 + 1: forward_shaped<512, 1>(p, vec, s); break;
-        case 512 * 8 + 2: forward_shaped<512, 2>(p, vec, s); break;
-        case 1024 * 8 + 2: forward_shaped<1024, 2>(p, vec, s); break;
-        case 1024 * 8 + 4: forward_shaped<1024, 4>(p, vec, s); break;
+    switch (shape.threads * 64 + shape.elements) {
+        case 32 * 64 + 8: forward_shaped<32, 8>(p, group, dev.sm_count, s); break;
+        case 32 * 64 + 16: forward_shaped<32, 16>(p, group, dev.sm_count, s); break;
+        case 32 * 64 + 24: forward_shaped<32, 24>(p, group, dev.sm_count, s); break;
+        case 32 * 64 + 32: forward_shaped<32, 32>(p, group, dev.sm_count, s); break;
+        case 256 * 64 + 8: forward_shaped<256, 8>(p, group, dev.sm_count, s); break;
+        case 512 * 64 + 8: forward_shaped<512, 8>(p, group, dev.sm_count, s); break;
+        case 512 * 64 + 12: forward_shaped<512, 12>(p, group, dev.sm_count, s); break;
+        case 512 * 64 + 16: forward_shaped<512, 16>(p, group, dev.sm_count, s); break;
+        case 1024 * 64 + 16: forward_shaped<1024, 16>(p, group, dev.sm_count, s); break;
         default: layer_norm_wide_kernel<<<static_cast<unsigned>(a.rows), kWideThreads, 0, s>>>(p); break;
     }
     return launched("layer_norm_kernel launch", err);
@@ -543,19 +814,22 @@ int layer_norm_backward_launch(cudaStream_t s, const snb_layer_norm_args& a, std
     p.y_stride = static_cast<int64_t>(a.input_grad_stride);
     p.y_bf16 = p.x_bf16;
     p.sums = static_cast<float*>(a.workspace);
-    const bool vec = vectors(a.input, a.input_stride, a.cols, a.input_type) &&
-                     vectors(a.output_grad, a.output_grad_stride, a.cols, a.output_grad_type) &&
-                     vectors(a.input_grad, a.input_grad_stride, a.cols, a.input_type) && aligned16(a.gain);
+    const bool whole = pieces16(a.input, a.input_stride, a.cols, a.input_type) &&
+                       pieces16(a.output_grad, a.output_grad_stride, a.cols, a.output_grad_type) &&
+                       pieces16(a.input_grad, a.input_grad_stride, a.cols, a.input_type) && aligned16(a.gain);
+    const int group = !whole ? 1 : p.x_bf16 && p.dy_bf16 ? 8 : 4;
     const unsigned grid = static_cast<unsigned>(backward_grid(a.rows, a.cols, dev.sm_count));
     const Shape shape = shape_of(a.cols, true);
-    switch (shape.threads * 8 + shape.pieces) {
-        case 32 * 8 + 1: backward_shaped<32, 1>(p, vec, grid, s); break;
-        case 32 * 8 + 2: backward_shaped<32, 2>(p, vec, grid, s); break;
-        case 32 * 8 + 3: backward_shaped<32, 3>(p, vec, grid, s); break;
-        case 32 * 8 + 4: backward_shaped<32, 4>(p, vec, grid, s); break;
-        case 256 * 8 + 1: backward_shaped<256, 1>(p, vec, grid, s); break;
-        case 512 * 8 + 1: backward_shaped<512, 1>(p, vec, grid, s); break;
-        case 512 * 8 + 2: backward_shaped<512, 2>(p, vec, grid, s); break;
+    switch (shape.threads * 64 + shape.elements) {
+        case 32 * 64 + 8: backward_shaped<32, 8>(p, group, grid, s); break;
+        case 32 * 64 + 16: backward_shaped<32, 16>(p, group, grid, s); break;
+        case 32 * 64 + 24: backward_shaped<32, 24>(p, group, grid, s); break;
+        case 128 * 64 + 8: backward_shaped<128, 8>(p, group, grid, s); break;
+        case 256 * 64 + 8: backward_shaped<256, 8>(p, group, grid, s); break;
+        case 256 * 64 + 16: backward_shaped<256, 16>(p, group, grid, s); break;
+        case 256 * 64 + 20: backward_shaped<256, 20>(p, group, grid, s); break;
+        case 256 * 64 + 24: backward_shaped<256, 24>(p, group, grid, s); break;
+        case 512 * 64 + 16: backward_shaped<512, 16>(p, group, grid, s); break;
         default:
             // The columns first: the input gradient may overwrite the output gradient.
             layer_norm_wide_columns_kernel<<<dim3(static_cast<unsigned>((a.cols + 255) / 256), grid), 256, 0, s>>>(p);
@@ -564,8 +838,18 @@ int layer_norm_backward_launch(cudaStream_t s, const snb_layer_norm_args& a, std
             break;
     }
     if ((rc = launched("layer_norm_backward_kernel launch", err)) != SNB_OK) return rc;
-    layer_norm_columns_kernel<<<dim3(static_cast<unsigned>((a.cols + 31) / 32), 2), 1024, 0, s>>>(
-        p.sums, grid, p.cols, a.gain_grad, a.bias_grad, a.accumulate != 0);
+    // Scheduled while the grid above drains; it waits for that grid before it reads.
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(static_cast<unsigned>((a.cols + 31) / 32), 2);
+    cfg.blockDim = dim3(1024);
+    cfg.stream = s;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, layer_norm_columns_kernel, static_cast<const float*>(p.sums), static_cast<int64_t>(grid),
+                       p.cols, a.gain_grad, a.bias_grad, a.accumulate != 0 ? 1 : 0);
     return launched("layer_norm_columns_kernel launch", err);
 }
 

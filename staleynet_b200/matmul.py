@@ -317,60 +317,57 @@ class Gpu:
             raise AssertionError(self.lib.snb_last_error().decode())
         check(code)
 
-    def _layer_norm_args(self, name, params, mean, inv_std, tensors, dense) -> _ffi.LayerNormArgs:
-        """snb_layer_norm_args: `tensors` {field: [rows, cols] tensor}, whose rows may be strided; `params` the [cols]
-        f32 vectors by field; `dense` every f32 vector, checked for its type and density."""
+    @staticmethod
+    def _norm_rows(name, field, t, rows, cols):
+        """(pointer, length, stride, type) of one [rows, cols] tensor of a layer norm, whose rows may be strided."""
         import torch
 
-        first = tensors["input"]
-        if first.dim() != 2:
-            raise AssertionError(f"{name}: input must be [rows, cols]")
-        rows, cols = first.shape
-        a = _ffi.LayerNormArgs(rows=rows, cols=cols, mean=mean.data_ptr(), inv_std=inv_std.data_ptr(),
-                               params_len=cols, stats_len=min(mean.numel(), inv_std.numel()))
-        for t in dense:
+        if not t.is_cuda:
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "tensors must live in CUDA device memory")
+        if t.dim() != 2 or t.shape[0] != rows or t.shape[1] != cols:
+            raise AssertionError(f"{name}: {field} shape")
+        kind = _ffi.TYPE_BF16 if t.dtype is torch.bfloat16 else _ffi.TYPE_F32
+        if kind == _ffi.TYPE_F32 and t.dtype is not torch.float32:
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: {field} must be float32 or bfloat16")
+        stride, unit = t.stride()
+        if cols > 1 and unit != 1:
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: {field}'s rows must be contiguous")
+        if rows <= 1:
+            stride = cols
+        return t.data_ptr(), (rows - 1) * stride + cols if rows else 0, stride, kind
+
+    @staticmethod
+    def _norm_vectors(name, cols, params, stats):
+        """(params_len, stats_len) of the dense f32 vectors of a layer norm."""
+        import torch
+
+        params_len = cols
+        for t in params:
+            if t.numel() != cols:
+                params_len = t.numel()
+        for t in params + stats:
             if not t.is_cuda:
                 raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "tensors must live in CUDA device memory")
             if t.dtype is not torch.float32 or not t.is_contiguous():
                 raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: parameters and statistics must be dense float32")
-        for field, t in params.items():
-            if t is not None:
-                if t.numel() != cols:
-                    a.params_len = t.numel()
-                setattr(a, field, t.data_ptr())
-        for field, t in tensors.items():
-            if not t.is_cuda:
-                raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "tensors must live in CUDA device memory")
-            if t.shape != first.shape:
-                raise AssertionError(f"{name}: {field} shape")
-            if t.dtype is torch.bfloat16:
-                kind = _ffi.TYPE_BF16
-            elif t.dtype is torch.float32:
-                kind = _ffi.TYPE_F32
-            else:
-                raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: {field} must be float32 or bfloat16")
-            step, unit = t.stride()
-            if cols > 1 and unit != 1:
-                raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: {field}'s rows must be contiguous")
-            stride = step if rows > 1 else cols
-            setattr(a, field, t.data_ptr())
-            setattr(a, field + "_stride", stride)
-            setattr(a, field + "_len", (rows - 1) * stride + cols if rows else 0)
-            if field != "input_grad":
-                setattr(a, field + "_type", kind)
-            elif t.dtype is not first.dtype:
-                raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: input_grad must have the input's dtype")
-        return a
+        return params_len, min(stats[0].numel(), stats[1].numel())
 
     def layer_norm_forward(self, input, gain, bias, output, mean, inv_std, epsilon: float) -> None:
         """Layer norm (snb_layer_norm_forward): rows of input [rows, cols] (f32 or bf16) to zero mean and unit variance,
         times gain, plus bias (or None), into output (f32 or bf16); mean and inv_std ([rows] f32) are kept for the
         backward pass."""
-        vectors = (gain, mean, inv_std) if bias is None else (gain, bias, mean, inv_std)
-        a = self._layer_norm_args("layer_norm_forward", {"gain": gain, "bias": bias}, mean, inv_std,
-                                  {"input": input, "output": output}, vectors)
-        a.epsilon = epsilon
-        check(self.lib.snb_layer_norm_forward(self._stream_handle(), ctypes.byref(a)))
+        name = "layer_norm_forward"
+        if input.dim() != 2:
+            raise AssertionError(f"{name}: input must be [rows, cols]")
+        rows, cols = input.shape
+        x = self._norm_rows(name, "input", input, rows, cols)
+        y = self._norm_rows(name, "output", output, rows, cols)
+        lens = self._norm_vectors(name, cols, (gain,) if bias is None else (gain, bias), (mean, inv_std))
+        a = _ffi.LayerNormArgs(rows, cols, *x, epsilon, gain.data_ptr(), None if bias is None else bias.data_ptr(),
+                               lens[0], mean.data_ptr(), inv_std.data_ptr(), lens[1], *y)
+        code = self.lib.snb_layer_norm_forward(self._stream_handle(), ctypes.byref(a))
+        if code != _ffi.OK:
+            check(code)
 
     def layer_norm_workspace(self, rows: int, cols: int) -> int:
         """Bytes of workspace that layer_norm_backward needs (snb_layer_norm_workspace)."""
@@ -383,14 +380,25 @@ class Gpu:
         """Layer norm's backward pass (snb_layer_norm_backward): input_grad (of the input's dtype), and gain_grad and
         bias_grad (f32, bias_grad or None) overwritten or, with WriteMode.ACCUMULATE, added to. mean and inv_std as
         layer_norm_forward wrote them."""
-        vectors = (gain, mean, inv_std, gain_grad) if bias_grad is None else (gain, mean, inv_std, gain_grad, bias_grad)
+        name = "layer_norm_backward"
+        if input.dim() != 2:
+            raise AssertionError(f"{name}: input must be [rows, cols]")
+        rows, cols = input.shape
+        x = self._norm_rows(name, "input", input, rows, cols)
+        dy = self._norm_rows(name, "output_grad", output_grad, rows, cols)
+        dx = self._norm_rows(name, "input_grad", input_grad, rows, cols)
+        if dx[3] != x[3]:
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"{name}: input_grad must have the input's dtype")
         _require_cuda(workspace)
-        a = self._layer_norm_args("layer_norm_backward", {"gain": gain, "gain_grad": gain_grad, "bias_grad": bias_grad},
-                                  mean, inv_std, {"input": input, "output_grad": output_grad, "input_grad": input_grad},
-                                  vectors)
-        a.accumulate = write.flag()
-        a.workspace, a.workspace_len = workspace.data_ptr(), workspace.numel() * workspace.element_size()
-        check(self.lib.snb_layer_norm_backward(self._stream_handle(), ctypes.byref(a)))
+        lens = self._norm_vectors(name, cols, (gain, gain_grad) if bias_grad is None else (gain, gain_grad, bias_grad),
+                                  (mean, inv_std))
+        a = _ffi.LayerNormArgs(rows, cols, *x, 0.0, gain.data_ptr(), None, lens[0], mean.data_ptr(), inv_std.data_ptr(),
+                               lens[1], None, 0, 0, 0, dy[3], *dy[:3], *dx[:3], gain_grad.data_ptr(),
+                               None if bias_grad is None else bias_grad.data_ptr(), write.flag(), 0,
+                               workspace.data_ptr(), workspace.numel() * workspace.element_size())
+        code = self.lib.snb_layer_norm_backward(self._stream_handle(), ctypes.byref(a))
+        if code != _ffi.OK:
+            check(code)
 
     def rms_norm_stats(self, input, epsilon: float, inv_rms, gain=None, output=None) -> None:
         """snb_rms_norm_stats: 1/rms per row of input (f32 or bf16), and the normalised rows when `output` is
