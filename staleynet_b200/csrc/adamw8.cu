@@ -33,6 +33,7 @@ namespace {
 constexpr int kBlock = 256;             // elements that share a scale
 constexpr int kWarps = 8;               // warps of a thread block
 constexpr int kChunk = 4 * kWarps * kBlock;  // elements that a thread block takes at a time
+constexpr int kStepBlocks = 3;          // thread blocks of the step that are resident on an SM (80 registers a thread)
 constexpr int kMaxTensors = 256;        // of one launch (its table is a kernel parameter)
 constexpr int kSumBlocks = 592;         // thread blocks of the norm's sum, and partial sums of one launch
 constexpr uint64_t kGolden = 0x9E3779B97F4A7C15ull;
@@ -66,11 +67,26 @@ __device__ __forceinline__ bool multiple(const void* p, uint32_t n) {
     return (reinterpret_cast<uintptr_t>(p) & (n - 1)) == 0;
 }
 
+// The arithmetic goes on pairs of elements with packed f32x2 instructions: a step costs about as many instructions as its
+// memory traffic leaves time for. Their constants come as pairs from the kernel's parameters, where an instruction can
+// take them from; pairs of literals would be assembled in registers at each use.
+__device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
+
+struct Constants {
+    float2 first, second;       // 1 / 127^2, 1 / 255^2
+    float2 integer, code, one;  // -2^23, -2^23 - 128, 1
+    float2 round;               // 2^23
+    float2 guess1, guess2;      // 127 and 255, less 2^-20 of them
+    float2 unit, unit_shift;    // 2^-16, 2^-17 - 128
+};
+
 // The share of its block's scale that a magnitude code stands for.
-__device__ __forceinline__ float first_level(float q) { return __fmul_rn(__fmul_rn(q, q), 1.0f / 16129.0f); }
-__device__ __forceinline__ float second_level(float q) {
-    const float s = __fmul_rn(__fmul_rn(q, q), 1.0f / 65025.0f);
-    return __fmul_rn(s, s);
+__device__ __forceinline__ float2 first_level(float2 q, const Constants& k) {
+    return __fmul2_rn(__fmul2_rn(q, q), k.first);
+}
+__device__ __forceinline__ float2 second_level(float2 q, const Constants& k) {
+    const float2 s = __fmul2_rn(__fmul2_rn(q, q), k.second);
+    return __fmul2_rn(s, s);
 }
 
 __device__ __forceinline__ float sqrt_fast(float x) {
@@ -79,33 +95,65 @@ __device__ __forceinline__ float sqrt_fast(float x) {
     return y;
 }
 
-// The code of `share` (a magnitude over its block's scale): q is the last level up to it, found from `guess`, which may
-// be one level off, and kept below the last level; the upper neighbour is taken if the random threshold between the two
-// lies below the share. NaN gives 0.
+// The larger of two magnitudes, NaN if either is.
+__device__ __forceinline__ float max_or_nan(float a, float b) {
+    float y;
+    asm("max.NaN.f32 %0, %1, %2;" : "=f"(y) : "f"(a), "f"(fabsf(b)));
+    return y;
+}
+
+// Floats 2^23 + n are integers n in their low bits: codes go in and out of f32 by additions, not conversions.
+constexpr float kInteger = 8388608.0f;
+
+// (b + 0.5) / 65536 for the 16 random bits b of one half of each word: 2^23 + b, scaled and shifted in one exact operation.
+template <int HALF>
+__device__ __forceinline__ float2 random_units(uint32_t bits0, uint32_t bits1, const Constants& k) {
+    const float2 b = make_float2(__uint_as_float(__byte_perm(bits0, 0x4B000000u, HALF == 0 ? 0x7410 : 0x7432)),
+                                 __uint_as_float(__byte_perm(bits1, 0x4B000000u, HALF == 0 ? 0x7410 : 0x7432)));
+    return __ffma2_rn(b, k.unit, k.unit_shift);
+}
+
+// The codes of a pair of shares (magnitudes over their block's scale), in the low bits of the results. q is the last
+// level up to a share, at most one below the highest; its upper neighbour is taken if the random threshold between the two
+// lies below the share. `guess` is q before it is rounded down, from approximate roots (2^-22) made smaller by 2^-20: it
+// gives q or, for shares that close above a level, q - 1, which the comparison with the upper level shows. Shares of
+// 0.9999 and more belong to the last step whatever it says.
 template <typename Level>
-__device__ __forceinline__ float encode(float share, float guess, float most, uint32_t bits16, Level level) {
-    float q = share > 0.0f ? fminf(floorf(guess), most - 1.0f) : 0.0f;
-    float low = level(q), high = level(q + 1.0f);
-    if (low > share && q > 0.0f) {
-        q -= 1.0f;
-        high = low;
+__device__ __forceinline__ uint2 encode(float2 share, float2 guess, float2 u, const Constants& k, Level level) {
+    float2 r = __fadd2_rd(guess, k.round);
+    float2 q = __fadd2_rn(r, k.integer);
+    float2 low = level(q), high = level(__fadd2_rn(q, k.one));
+    const bool more_x = high.x <= fminf(share.x, 0.9999f), more_y = high.y <= fminf(share.y, 0.9999f);
+    if (more_x || more_y) {
+        r = __fadd2_rn(r, make_float2(more_x ? 1.0f : 0.0f, more_y ? 1.0f : 0.0f));
+        q = __fadd2_rn(r, k.integer);
         low = level(q);
-    } else if (high <= share && q < most - 1.0f) {
-        q += 1.0f;
-        low = high;
-        high = level(q + 1.0f);
+        high = level(__fadd2_rn(q, k.one));
     }
-    const float u = __fmul_rn(__fadd_rn(static_cast<float>(bits16), 0.5f), 1.0f / 65536.0f);
-    const float threshold = __fadd_rn(low, __fmul_rn(u, __fsub_rn(high, low)));
-    return threshold < share ? q + 1.0f : q;
+    const float2 step = __fadd2_rn(high, make_float2(-low.x, -low.y));
+    const float2 threshold = __fadd2_rn(low, __fmul2_rn(u, step));
+    return make_uint2(__float_as_uint(r.x) + (threshold.x < share.x ? 1u : 0u),
+                      __float_as_uint(r.y) + (threshold.y < share.y ? 1u : 0u));
+}
+
+// Byte k of a word of codes as a float: as it is, or of a word whose sign bits were flipped, as a signed value.
+__device__ __forceinline__ float code_value(uint32_t word, int k) {
+    return __uint_as_float(__byte_perm(word, 0x4B000000u, 0x7540 + k));
 }
 
 // (scale, 1 / scale) of a block whose largest magnitude has these bits (as integers magnitudes order like floats, with
-// infinity and NaN above all others: a block that holds one decodes to NaN). Subnormal scales count as 0.
+// infinity and NaN above all others). A block that holds one of those gets NaN, so that all of it decodes to NaN, whatever
+// its codes. Subnormal scales count as 0.
 __device__ __forceinline__ float2 scale_of(uint32_t bits) {
-    const float s = __uint_as_float(bits);
-    if (s < 1.17549435e-38f) return make_float2(0.0f, 0.0f);
-    return make_float2(s, s > 0.0f ? __frcp_rn(s) : 0.0f);
+    if (bits >= 0x7F800000u) return make_float2(__uint_as_float(0x7FFFFFFFu), 0.0f);
+    if (bits < 0x00800000u) return make_float2(0.0f, 0.0f);
+    return make_float2(__uint_as_float(bits), __frcp_rn(__uint_as_float(bits)));
+}
+
+__device__ __forceinline__ float reciprocal_fast(float x) {
+    float y;
+    asm("rcp.approx.ftz.f32 %0, %1;" : "=f"(y) : "f"(x));
+    return y;
 }
 
 // SplitMix64's output for a state.
@@ -174,8 +222,9 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_norm_kernel(const __grid_c
 }
 
 struct StepParams {
-    float learning_rate, beta1, beta2, one_minus_beta1, one_minus_beta2, epsilon;
-    float first_correction, second_correction;  // 1 / (1 - beta^step)
+    float2 minus_learning_rate, beta1, beta2, one_minus_beta1, one_minus_beta2, epsilon;
+    float2 first_correction, second_correction;  // 1 / (1 - beta^step)
+    Constants k;
     float max_norm;
     uint64_t seed;
     const double* partials;
@@ -183,7 +232,7 @@ struct StepParams {
     double* square_sum;
 };
 
-__global__ void __launch_bounds__(32 * kWarps) adamw8_step_kernel(const __grid_constant__ Table m, const StepParams a) {
+__global__ void __launch_bounds__(32 * kWarps, kStepBlocks) adamw8_step_kernel(const __grid_constant__ Table m, const StepParams a) {
     // Every thread block adds the norm's partial sums in the same order.
     double sum = 0.0;
     for (int i = threadIdx.x; i < a.partial_count; i += 32 * kWarps) sum += a.partials[i];
@@ -238,49 +287,34 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_step_kernel(const __grid_c
                 }
             }
             const float s1 = x.first_scale[at / kBlock], s2 = x.second_scale[at / kBlock];
-            float mean[8], variance[8];
-            uint32_t top1 = 0, top2 = 0;
+            float2 mean[4], variance[4];
+            float top1 = 0.0f, top2 = 0.0f;
+            c1[0] ^= 0x80808080u;
+            c1[1] ^= 0x80808080u;
 #pragma unroll
-            for (int j = 0; j < 8; ++j) {
-                const float q1 = static_cast<float>(static_cast<int8_t>(c1[j >> 2] >> (8 * (j & 3))));
-                const float q2 = static_cast<float>((c2[j >> 2] >> (8 * (j & 3))) & 0xFFu);
-                const float gj = __fmul_rn(g[j], clip);
-                const float old1 = __fmul_rn(__fmul_rn(__fmul_rn(q1, fabsf(q1)), 1.0f / 16129.0f), s1);
-                const float old2 = __fmul_rn(second_level(q2), s2);
-                mean[j] = __fadd_rn(__fmul_rn(old1, a.beta1), __fmul_rn(gj, a.one_minus_beta1));
-                variance[j] = __fadd_rn(__fmul_rn(old2, a.beta2), __fmul_rn(__fmul_rn(gj, a.one_minus_beta2), gj));
-                top1 = max(top1, __float_as_uint(mean[j]) & 0x7FFFFFFFu);
-                top2 = max(top2, __float_as_uint(variance[j]) & 0x7FFFFFFFu);
-                // The update itself decides no code: approximate root and quotient (2^-22) far below its own step.
-                const float root = sqrt_fast(variance[j] * a.second_correction) + a.epsilon;
-                const float update = __fdividef(mean[j] * a.first_correction, root) + x.weight_decay * w[j];
-                w[j] -= a.learning_rate * update;
+            for (int j = 0; j < 4; ++j) {  // elements 2j and 2j + 1
+                const int b = 2 * j & 3;
+                const float2 q1 = __fadd2_rn(make_float2(code_value(c1[j >> 1], b), code_value(c1[j >> 1], b + 1)), a.k.code);
+                const float2 q2 = __fadd2_rn(make_float2(code_value(c2[j >> 1], b), code_value(c2[j >> 1], b + 1)), a.k.integer);
+                const float2 gj = __fmul2_rn(make_float2(g[2 * j], g[2 * j + 1]), both(clip));
+                const float2 signed_square = make_float2(__fmul_rn(q1.x, fabsf(q1.x)), __fmul_rn(q1.y, fabsf(q1.y)));
+                const float2 old1 = __fmul2_rn(__fmul2_rn(signed_square, a.k.first), both(s1));
+                const float2 old2 = __fmul2_rn(second_level(q2, a.k), both(s2));
+                mean[j] = __fadd2_rn(__fmul2_rn(old1, a.beta1), __fmul2_rn(gj, a.one_minus_beta1));
+                variance[j] = __fadd2_rn(__fmul2_rn(old2, a.beta2), __fmul2_rn(__fmul2_rn(gj, a.one_minus_beta2), gj));
+                top1 = max_or_nan(max_or_nan(top1, mean[j].x), mean[j].y);
+                top2 = max_or_nan(max_or_nan(top2, variance[j].x), variance[j].y);
+                // The update itself decides no code: approximate root and reciprocal (2^-22) far below its own step.
+                const float2 vh = __fmul2_rn(variance[j], a.second_correction);
+                const float2 root = __fadd2_rn(make_float2(sqrt_fast(vh.x), sqrt_fast(vh.y)), a.epsilon);
+                const float2 mh = __fmul2_rn(mean[j], a.first_correction);
+                const float2 old = make_float2(w[2 * j], w[2 * j + 1]);
+                const float2 rate = __fmul2_rn(mh, make_float2(reciprocal_fast(root.x), reciprocal_fast(root.y)));
+                const float2 next = __ffma2_rn(a.minus_learning_rate, __ffma2_rn(both(x.weight_decay), old, rate), old);
+                w[2 * j] = next.x;
+                w[2 * j + 1] = next.y;
             }
-            const float2 n1 = scale_of(__reduce_max_sync(0xffffffffu, top1));
-            const float2 n2 = scale_of(__reduce_max_sync(0xffffffffu, top2));
-            c1[0] = c1[1] = c2[0] = c2[1] = 0;
-#pragma unroll
-            for (int j = 0; j < 8; j += 2) {
-                const uint64_t draw = x.first_draw + static_cast<uint64_t>(at + element_of(lane, j)) / 2 + 1;
-                const uint64_t bits = mix(a.seed + draw * kGolden);
-#pragma unroll
-                for (int k = 0; k < 2; ++k) {
-                    const uint32_t b = static_cast<uint32_t>(bits >> (32 * k));
-                    const float share1 = __fmul_rn(fabsf(mean[j + k]), n1.y);
-                    const float share2 = __fmul_rn(variance[j + k], n2.y);
-                    const float q1 = encode(share1, 127.0f * sqrt_fast(share1), 127.0f, b & 0xFFFFu, first_level);
-                    float q2 = encode(share2, 255.0f * sqrt_fast(sqrt_fast(share2)), 255.0f, b >> 16, second_level);
-                    if (variance[j + k] > 0.0f) q2 = fmaxf(q2, 1.0f);
-                    const int code1 = mean[j + k] < 0.0f ? -static_cast<int>(q1) : static_cast<int>(q1);
-                    const int shift = 8 * ((j + k) & 3);
-                    c1[j >> 2] |= (static_cast<uint32_t>(code1) & 0xFFu) << shift;
-                    c2[j >> 2] |= static_cast<uint32_t>(q2) << shift;
-                }
-            }
-            if (lane == 0) {
-                x.first_scale[at / kBlock] = n1.x;
-                x.second_scale[at / kBlock] = n2.x;
-            }
+            // The parameter leaves now, so that its registers serve the encoding.
             if (whole) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -290,8 +324,6 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_step_kernel(const __grid_c
                     if (x.shadow != nullptr)
                         *reinterpret_cast<uint2*>(x.shadow + e) = make_uint2(bf16_pair(w[4 * h], w[4 * h + 1]),
                                                                              bf16_pair(w[4 * h + 2], w[4 * h + 3]));
-                    *reinterpret_cast<uint32_t*>(x.first + e) = c1[h];
-                    *reinterpret_cast<uint32_t*>(x.second + e) = c2[h];
                 }
             } else {
 #pragma unroll
@@ -300,6 +332,57 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_step_kernel(const __grid_c
                     if (e >= count) continue;
                     x.parameter[e] = w[j];
                     if (x.shadow != nullptr) x.shadow[e] = static_cast<uint16_t>(bf16_pair(w[j], 0.0f));
+                }
+            }
+            const float2 n1 = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top1) & 0x7FFFFFFFu));
+            const float2 n2 = scale_of(__reduce_max_sync(0xffffffffu, __float_as_uint(top2) & 0x7FFFFFFFu));
+            // States of the lane's draws: elements 2j and 2j + 1 share one; pairs 0 and 1 are 64 draws before 2 and 3.
+            const uint64_t state = a.seed + (x.first_draw + static_cast<uint64_t>(at / 2 + 2 * lane) + 1) * kGolden;
+            uint32_t code1[8], code2[8];
+#pragma unroll
+            for (int j = 0; j < 4; ++j) {
+                const uint64_t bits = mix(state + ((j & 1) + (j >> 1) * 64) * kGolden);
+                const uint32_t b0 = static_cast<uint32_t>(bits), b1 = static_cast<uint32_t>(bits >> 32);
+                const float2 share1 = __fmul2_rn(make_float2(fabsf(mean[j].x), fabsf(mean[j].y)), both(n1.y));
+                const float2 share2 = __fmul2_rn(variance[j], both(n2.y));
+                const float2 guess1 = __fmul2_rn(make_float2(sqrt_fast(share1.x), sqrt_fast(share1.y)), a.k.guess1);
+                const float2 guess2 = __fmul2_rn(
+                    make_float2(sqrt_fast(sqrt_fast(share2.x)), sqrt_fast(sqrt_fast(share2.y))), a.k.guess2);
+                const uint2 e1 = encode(share1, guess1, random_units<0>(b0, b1, a.k), a.k,
+                                        [&](float2 q) { return first_level(q, a.k); });
+                const uint2 e2 = encode(share2, guess2, random_units<1>(b0, b1, a.k), a.k,
+                                        [&](float2 q) { return second_level(q, a.k); });
+                // m's sign; v's lowest code above 0.
+                const uint32_t m0 = static_cast<uint32_t>(static_cast<int32_t>(__float_as_uint(mean[j].x)) >> 31);
+                const uint32_t m1 = static_cast<uint32_t>(static_cast<int32_t>(__float_as_uint(mean[j].y)) >> 31);
+                code1[2 * j] = (e1.x ^ m0) - m0;
+                code1[2 * j + 1] = (e1.y ^ m1) - m1;
+                code2[2 * j] = max(e2.x, variance[j].x > 0.0f ? 0x4B000001u : 0x4B000000u);
+                code2[2 * j + 1] = max(e2.y, variance[j].y > 0.0f ? 0x4B000001u : 0x4B000000u);
+            }
+#pragma unroll
+            for (int h = 0; h < 2; ++h) {
+                c1[h] = __byte_perm(__byte_perm(code1[4 * h], code1[4 * h + 1], 0x0040),
+                                    __byte_perm(code1[4 * h + 2], code1[4 * h + 3], 0x0040), 0x5410);
+                c2[h] = __byte_perm(__byte_perm(code2[4 * h], code2[4 * h + 1], 0x0040),
+                                    __byte_perm(code2[4 * h + 2], code2[4 * h + 3], 0x0040), 0x5410);
+            }
+            if (lane == 0) {
+                x.first_scale[at / kBlock] = n1.x;
+                x.second_scale[at / kBlock] = n2.x;
+            }
+            if (whole) {
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t e = at + element_of(lane, 4 * h);
+                    *reinterpret_cast<uint32_t*>(x.first + e) = c1[h];
+                    *reinterpret_cast<uint32_t*>(x.second + e) = c2[h];
+                }
+            } else {
+#pragma unroll
+                for (int j = 0; j < 8; ++j) {
+                    const int64_t e = at + element_of(lane, j);
+                    if (e >= count) continue;
                     x.first[e] = static_cast<int8_t>(c1[j >> 2] >> (8 * (j & 3)));
                     x.second[e] = static_cast<uint8_t>(c2[j >> 2] >> (8 * (j & 3)));
                 }
@@ -332,7 +415,10 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_moments_kernel(const __gri
                 const float q = static_cast<float>(c);
                 return __fmul_rn(__fmul_rn(__fmul_rn(q, fabsf(q)), 1.0f / 16129.0f), s1);
             };
-            auto value2 = [&](uint32_t c) { return __fmul_rn(second_level(static_cast<float>(c)), s2); };
+            auto value2 = [&](uint32_t c) {
+                const float q = static_cast<float>(c), root = __fmul_rn(__fmul_rn(q, q), 1.0f / 65025.0f);
+                return __fmul_rn(__fmul_rn(root, root), s2);
+            };
             if (aligned && at + kBlock <= count) {
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
@@ -410,14 +496,25 @@ int adamw8_step_launch(cudaStream_t s, const snb_adamw8_tensor* tensors, uint64_
         return SNB_ERR_CUDA;
     }
     StepParams a{};
-    a.learning_rate = h.learning_rate;
-    a.beta1 = h.beta1;
-    a.beta2 = h.beta2;
-    a.one_minus_beta1 = 1.0f - h.beta1;
-    a.one_minus_beta2 = 1.0f - h.beta2;
-    a.epsilon = h.epsilon;
-    a.first_correction = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(h.beta1), h.step)));
-    a.second_correction = static_cast<float>(1.0 / (1.0 - std::pow(static_cast<double>(h.beta2), h.step)));
+    auto pair = [](double v) { return make_float2(static_cast<float>(v), static_cast<float>(v)); };
+    a.minus_learning_rate = pair(-h.learning_rate);
+    a.beta1 = pair(h.beta1);
+    a.beta2 = pair(h.beta2);
+    a.one_minus_beta1 = pair(1.0f - h.beta1);
+    a.one_minus_beta2 = pair(1.0f - h.beta2);
+    a.epsilon = pair(h.epsilon);
+    a.first_correction = pair(1.0 / (1.0 - std::pow(static_cast<double>(h.beta1), h.step)));
+    a.second_correction = pair(1.0 / (1.0 - std::pow(static_cast<double>(h.beta2), h.step)));
+    a.k.first = pair(1.0f / 16129.0f);
+    a.k.second = pair(1.0f / 65025.0f);
+    a.k.round = pair(kInteger);
+    a.k.integer = pair(-kInteger);
+    a.k.code = pair(-kInteger - 128.0f);
+    a.k.one = pair(1.0);
+    a.k.guess1 = pair(127.0 * (1.0 - 0x1p-20));
+    a.k.guess2 = pair(255.0 * (1.0 - 0x1p-20));
+    a.k.unit = pair(0x1p-16);
+    a.k.unit_shift = pair(0x1p-17 - 128.0);
     a.max_norm = max_gradient_norm;
     a.seed = seed;
     a.partials = partials;
@@ -427,7 +524,7 @@ int adamw8_step_launch(cudaStream_t s, const snb_adamw8_tensor* tensors, uint64_
         if (n > kMaxTensors) fill(&table, tensors, i, n);
         const int64_t chunks = table.chunk_start[table.n];
         if (chunks == 0) continue;
-        const int64_t blocks = std::min<int64_t>(chunks, 4ll * dev.sm_count);
+        const int64_t blocks = std::min<int64_t>(chunks, static_cast<int64_t>(kStepBlocks) * dev.sm_count);
         adamw8_step_kernel<<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(table, a);
         if ((rc = launched("adamw8_step_kernel launch", err)) != SNB_OK) return rc;
     }
