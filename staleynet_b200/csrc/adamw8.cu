@@ -10,8 +10,9 @@
 // would divide that m by epsilon.
 //   The random bits of elements 2i and 2i + 1 of a tensor are the halves of output first_draw + i + 1 of the reference's
 // SplitMix64 (Random::new(seed), crates/staleynet-model/src/random.rs:27-50): 16 bits for each moment.
-//   Everything that decides a code is written with explicitly rounded f32 operations, so codes do not depend on how the
-// compiler contracts them.
+//   Everything that decides a code is made of f32 operations that are rounded one by one, so codes do not depend on the
+// compiler. (It contracts packed products and sums to multiply-adds, even where both ask for their own rounding: sums of
+// products are therefore scalar additions, sum_of.)
 //
 // Step. As the reference's (kernels/optimizer.rs:57-70) on g = gradient times the clip factor max_norm / norm; the norm is
 // that of all tensors together, its squares summed in f64 in a fixed order, so steps are the same from run to run.
@@ -72,6 +73,8 @@ __device__ __forceinline__ bool multiple(const void* p, uint32_t n) {
 // take them from; pairs of literals would be assembled in registers at each use.
 __device__ __forceinline__ float2 both(float v) { return make_float2(v, v); }
 
+__device__ __forceinline__ float2 sum_of(float2 a, float2 b) { return make_float2(__fadd_rn(a.x, b.x), __fadd_rn(a.y, b.y)); }
+
 struct Constants {
     float2 first, second;       // 1 / 127^2, 1 / 255^2
     float2 integer, code, one;  // -2^23, -2^23 - 128, 1
@@ -130,8 +133,8 @@ __device__ __forceinline__ uint2 encode(float2 share, float2 guess, float2 u, co
         low = level(q);
         high = level(__fadd2_rn(q, k.one));
     }
-    const float2 step = __fadd2_rn(high, make_float2(-low.x, -low.y));
-    const float2 threshold = __fadd2_rn(low, __fmul2_rn(u, step));
+    const float2 step = sum_of(high, make_float2(-low.x, -low.y));  // (levels are products)
+    const float2 threshold = sum_of(low, __fmul2_rn(u, step));
     return make_uint2(__float_as_uint(r.x) + (threshold.x < share.x ? 1u : 0u),
                       __float_as_uint(r.y) + (threshold.y < share.y ? 1u : 0u));
 }
@@ -300,8 +303,8 @@ __global__ void __launch_bounds__(32 * kWarps, kStepBlocks) adamw8_step_kernel(c
                 const float2 signed_square = make_float2(__fmul_rn(q1.x, fabsf(q1.x)), __fmul_rn(q1.y, fabsf(q1.y)));
                 const float2 old1 = __fmul2_rn(__fmul2_rn(signed_square, a.k.first), both(s1));
                 const float2 old2 = __fmul2_rn(second_level(q2, a.k), both(s2));
-                mean[j] = __fadd2_rn(__fmul2_rn(old1, a.beta1), __fmul2_rn(gj, a.one_minus_beta1));
-                variance[j] = __fadd2_rn(__fmul2_rn(old2, a.beta2), __fmul2_rn(__fmul2_rn(gj, a.one_minus_beta2), gj));
+                mean[j] = sum_of(__fmul2_rn(old1, a.beta1), __fmul2_rn(gj, a.one_minus_beta1));
+                variance[j] = sum_of(__fmul2_rn(old2, a.beta2), __fmul2_rn(__fmul2_rn(gj, a.one_minus_beta2), gj));
                 top1 = max_or_nan(max_or_nan(top1, mean[j].x), mean[j].y);
                 top2 = max_or_nan(max_or_nan(top2, variance[j].x), variance[j].y);
                 // The update itself decides no code: approximate root and reciprocal (2^-22) far below its own step.

@@ -121,6 +121,50 @@ def _check_step(tensors, decays, max_norm, hyper, seed=99):
 HYPER = AdamWHyperparameters(3e-4, 0.9, 0.95, 1e-8, 0.0, 7)
 
 
+def _levels(q, power):
+    s = (q * q).float() * (1.0 / 16129.0 if power == 2 else 1.0 / 65025.0)
+    return s if power == 2 else s * s
+
+
+def _encode_f32(values, bits, power):
+    """The codes in elementary f32 operations, each rounded by itself (torch runs one at a time)."""
+    most = 127 if power == 2 else 255
+    blocks = values.view(-1, BLOCK)
+    scale = blocks.amax(1)
+    share = (blocks * (1.0 / scale)[:, None]).view(-1)
+    levels = _levels(torch.arange(most + 1, device="cuda", dtype=torch.int32), power)
+    q = (torch.searchsorted(levels, share, right=True) - 1).clamp(0, most - 1)
+    low, high = levels[q], levels[q + 1]
+    unit = (bits.float() + 0.5) * (1.0 / 65536.0)
+    threshold = low + unit * (high - low)
+    return q + (threshold < share), scale
+
+
+@pytest.mark.parametrize("gradient_type", [F32, BF16], ids=["f32", "bf16"])
+def test_codes_and_scales_are_those_of_f32_arithmetic_to_the_bit(gradient_type):
+    n, seed = BLOCK * 8000, 77
+    p, g, state, _ = _tensor(n, gradient_type, np.random.default_rng(21))
+    b1, b2 = _f(HYPER.beta1), _f(HYPER.beta2)
+    nb1, nb2 = _f(np.float32(1) - np.float32(b1)), _f(np.float32(1) - np.float32(b2))
+    q1, q2 = state[0].int(), state[2].int()
+    m = (torch.sign(q1) * _levels(q1, 2)).view(-1, BLOCK) * state[1][:, None]
+    v = _levels(q2, 4).view(-1, BLOCK) * state[3][:, None]
+    gf = g.float()
+    norm = torch.sqrt((g.double() ** 2).sum()).float()
+    gf = gf * (0.5 / norm)   # clipped: the norm is above 0.5
+    assert norm.item() > 0.5
+    m = m.view(-1) * b1 + gf * nb1
+    v = v.view(-1) * b2 + (gf * nb2) * gf
+    bits = torch.from_numpy(_bits(seed, 0, n)).cuda()
+    code1, scale1 = _encode_f32(m.abs(), bits & 0xFFFF, 2)
+    code2, scale2 = _encode_f32(v, bits >> 16, 4)
+    AdamW8(Gpu(0), [AdamW8Tensor(p, g, *state)]).step(HYPER, 0.5, seed)
+    torch.cuda.synchronize()
+    assert torch.equal(state[1], scale1) and torch.equal(state[3], scale2)
+    assert torch.equal(state[0].long(), torch.where(m < 0, -code1, code1))
+    assert torch.equal(state[2].long(), torch.where(v > 0, code2.clamp(min=1), code2))
+
+
 @pytest.mark.parametrize("gradient_type", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("n", [1, 2, 255, 256, 257, 1000, 8192, 8193, 300007])
 def test_one_tensor(n, gradient_type):
