@@ -81,6 +81,10 @@ struct TcParams {
     // side by side (tm_c 5-D: head_dim, capacity, heads, batch, P), columns (p * heads + h) * head_dim + d.
     int32_t a_heads, a_hd, a_time, a_toff;
     int32_t c_heads, c_hd, c_nheads, c_time, c_toff;
+    // Split f32 operands (tf32 kernels, count 1): A and B are each two planes, third coordinates 0 and 1 of their maps,
+    // the leading 11 significant bits and the rest. C += low(A) lead(B) + lead(A) low(B) + lead(A) lead(B) up to 2^-22:
+    // split s of K takes its share of the K slices of the first two products and then `lead_slices` slices of the third.
+    int32_t two_planes, a_low, b_low, lead_slices;
     // Vocabulary loss epilogues (TC_EPI_LSE, TC_EPI_SOFTMAX_GRAD): the product's columns are the classes
     // class_begin .. class_begin + N of a larger vocabulary.
     const uint32_t* targets;  // [M] class of each row; kNoTarget: the row has none
@@ -126,6 +130,7 @@ struct TcConfig {
 
 struct TcUnit {
     int32_t batch, m0, n0, kb_begin, kb_end, split;
+    int32_t low_begin, low_slices;  // two_planes: this unit's slices of the two products with a low part
     bool skip;  // every output of the tile is a masked score (SNB_CAUSAL_SKIP_MASKED_OUTPUT): no work at all
 };
 
@@ -154,6 +159,13 @@ __device__ __forceinline__ TcUnit tc_make_unit(const TcParams& p, int32_t split,
         // left[key, query] is zero for query < key - offset: start at the first query any row of the tile sees
         const int64_t first_query = static_cast<int64_t>(u.m0) - p.causal_offset;
         if (first_query > 0) u.kb_begin = max(u.kb_begin, static_cast<int32_t>(first_query / BK));
+    }
+    if (p.two_planes) {
+        const int64_t low = 2 * static_cast<int64_t>(p.k_blocks);
+        u.low_begin = static_cast<int32_t>(u.split * low / p.splits);
+        u.low_slices = static_cast<int32_t>((u.split + 1) * low / p.splits) - u.low_begin;
+        u.kb_begin = 0;
+        u.kb_end = u.low_slices + min(p.k_blocks - u.split * p.lead_slices, p.lead_slices);
     }
     // Keep at least one K slice (its masked contributions are zero) so the accumulator is always written.
     if (u.kb_begin >= u.kb_end) u.kb_begin = u.kb_end - 1;
@@ -457,6 +469,17 @@ __device__ __forceinline__ void load_a_slice(const TcParams& p, const CUtensorMa
             else tma_load_4d(sa + j * (BK * 128), tm_a, bar, m - h * p.a_hd, s, h, b);
         }
     }
+}
+
+// The K slice and the operands' planes of a unit's kb-th slice (two_planes).
+struct TcSlice {
+    int32_t k, a_plane, b_plane;
+};
+
+__device__ __forceinline__ TcSlice tc_slice(const TcParams& p, const TcUnit& u, int32_t kb) {
+    if (kb >= u.low_slices) return {u.split * p.lead_slices + kb - u.low_slices, 1 - p.a_low, 1 - p.b_low};
+    const int32_t v = u.low_begin + kb;
+    return v < p.k_blocks ? TcSlice{v, p.a_low, 1 - p.b_low} : TcSlice{v - p.k_blocks, 1 - p.a_low, p.b_low};
 }
 
 // Requests, on one lane, the auxiliary input of every column chunk an epilogue warp will stage for tile `u` (the
@@ -810,14 +833,20 @@ __global__ void __launch_bounds__(TC_THREADS, 1)
                     mbar_arrive_expect_tx(fb, Cfg::STAGE);
                     const uint32_t sa = smem_addr(ring + stage * Cfg::STAGE);
                     const uint32_t sb = sa + Cfg::STAGE_A;
-                    const int32_t k0 = kb * BK;
-                    load_a_slice<BK, MN_BOX, false>(p, &tm_a, sa, fb, u.m0, k0, ba);
+                    int32_t k0 = kb * BK, za = ba, zb = bb;
+                    if (!IS_BF16 && p.two_planes) {
+                        const TcSlice slice = tc_slice(p, u, kb);
+                        k0 = slice.k * BK;
+                        za = slice.a_plane;
+                        zb = slice.b_plane;
+                    }
+                    load_a_slice<BK, MN_BOX, false>(p, &tm_a, sa, fb, u.m0, k0, za);
                     if (!p.b_mn_major) {
-                        tma_load_3d(sb, &tm_b, fb, k0, u.n0, bb);
+                        tma_load_3d(sb, &tm_b, fb, k0, u.n0, zb);
                     } else {
 #pragma unroll
                         for (int j = 0; j < BN / MN_BOX; ++j)
-                            tma_load_3d(sb + j * (BK * 128), &tm_b, fb, u.n0 + j * MN_BOX, k0, bb);
+                            tma_load_3d(sb + j * (BK * 128), &tm_b, fb, u.n0 + j * MN_BOX, k0, zb);
                     }
                     if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1u; }
                     if (bias_pending && mbar_test_wait(smem_addr(&bias_empty[bbuf]), bpar)) {

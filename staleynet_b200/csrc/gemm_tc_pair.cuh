@@ -140,14 +140,20 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
                     const uint32_t fb = map_to_cta(fb_local, 0);
                     const uint32_t sa = smem_addr(ring + stage * Cfg::STAGE);
                     const uint32_t sb = sa + Cfg::STAGE_A;
-                    const int32_t k0 = kb * BK;
-                    load_a_slice<BK, MN_BOX, true>(p, &tm_a, sa, fb, m0, k0, ba);
+                    int32_t k0 = kb * BK, za = ba, zb = bb;
+                    if (!IS_BF16 && p.two_planes) {
+                        const TcSlice slice = tc_slice(p, u, kb);
+                        k0 = slice.k * BK;
+                        za = slice.a_plane;
+                        zb = slice.b_plane;
+                    }
+                    load_a_slice<BK, MN_BOX, true>(p, &tm_a, sa, fb, m0, k0, za);
                     if (!p.b_mn_major) {
-                        tma_load_3d_pair(sb, &tm_b, fb, k0, n0, bb);
+                        tma_load_3d_pair(sb, &tm_b, fb, k0, n0, zb);
                     } else {
 #pragma unroll
                         for (int j = 0; j < (BN / 2) / MN_BOX; ++j)
-                            tma_load_3d_pair(sb + j * (BK * 128), &tm_b, fb, n0 + j * MN_BOX, k0, bb);
+                            tma_load_3d_pair(sb + j * (BK * 128), &tm_b, fb, n0 + j * MN_BOX, k0, zb);
                     }
                     if (++stage == Cfg::STAGES) { stage = 0; phase ^= 1u; }
                     if (bias_pending && mbar_test_wait(smem_addr(&bias_empty[bbuf]), bpar)) {

@@ -31,7 +31,13 @@ struct GemmRequest {
     const snb_head_layout* a_heads;  // left operand read from its head-major form, or nullptr (snb_gemm_args)
     const snb_head_layout* c_heads;  // output written head-major, or nullptr
     int sm_budget;            // SMs the persistent grid may occupy (0: all; snb_set_sm_budget)
-    uint64_t max_split_inner; // longest sum of one split of K where K may be split (0: as the cost model has it)
+    uint64_t c_ld;            // elements between the output's rows (0: cols); other than cols on the tensor cores only,
+                              // for one plain product (no split of K, no tensor laid out like the output)
+    // f32 operands split in two planes (TF32 precision, count 1, f32 output, not deterministic): A and B point to the
+    // first plane, the second lies plane_stride elements after it, and `low` says which one holds the low parts.
+    // split_inner: longest sum of products of leading parts (see gemm_tc.cuh). 0: ordinary operands.
+    uint64_t split_inner, a_plane_stride, b_plane_stride;
+    int a_low, b_low;
 };
 
 struct DeviceInfo {

@@ -31,7 +31,8 @@ namespace snb {
 namespace {
 
 constexpr uint32_t kEmptyToken = 0xFFFFFFFFu;      // EMPTY_TOKEN (kernels/mod.rs:46)
-constexpr uint64_t kPieceBytes = 256ull << 20;     // bound of a piece of P (and of a packed piece of the weight)
+constexpr uint64_t kPieceBytes = 768ull << 20;     // bound of a piece of P
+constexpr uint64_t kWeightBytes = 256ull << 20;    // bound of a packed piece of the weight
 // Longest sum of f32 products on the tensor core, which cuts off the accumulator's lost bits at each instruction (8
 // products) instead of rounding: 2^-24 of the sum each time on average, always towards zero. Measured as the relative
 // error of a weight gradient over 1,021 rows: 2.5e-6 in one sum, 0.7e-6 in sums of 256 (0.6e-6 with f32 arithmetic).
@@ -59,15 +60,34 @@ struct PackParams {
     int32_t low;
 };
 
-__global__ void __launch_bounds__(256) pack_bf16_kernel(const PackParams p) {
-    const int64_t total = p.dst_rows * p.dst_cols;
-    const uint16_t* src = static_cast<const uint16_t*>(p.src);
-    uint16_t* dst = static_cast<uint16_t*>(p.dst);
-    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
-         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t i = e / p.dst_cols, j = e - i * p.dst_cols;
-        const bool live = i < p.rows && j < p.cols && (p.targets == nullptr || __ldg(p.targets + i) != kEmptyToken);
-        dst[i * p.dst_ld + j] = live ? src[i * p.src_ld + j] : 0;
+// Small kernels start while the kernel before them drains (programmatic launch) and wait for it here.
+__device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
+__device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
+
+// The three elementwise kernels take 4 columns (16 bytes of f32) a thread: blockDim.x threads along a row, blockDim.y rows
+// a block, rows in steps of the grid. `vec`: the side that is not in the workspace allows 4-element accesses.
+__device__ __forceinline__ bool has_target(const uint32_t* targets, int64_t row) {
+    return targets == nullptr || __ldg(targets + row) != kEmptyToken;
+}
+
+__global__ void __launch_bounds__(256) pack_bf16_kernel(const PackParams p, int vec) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; i < p.dst_rows;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        const bool live = i < p.rows && has_target(p.targets, i);
+        const uint16_t* src = static_cast<const uint16_t*>(p.src) + i * p.src_ld;
+        uint16_t* dst = static_cast<uint16_t*>(p.dst) + i * p.dst_ld;
+        for (int64_t j = 4 * threadIdx.x; j < p.dst_cols; j += 4 * blockDim.x) {
+            uint2 q = make_uint2(0, 0);
+            if (live && vec && j + 4 <= p.cols) {
+                q = __ldg(reinterpret_cast<const uint2*>(src + j));
+            } else if (live) {
+                uint32_t h[4];
+#pragma unroll
+                for (int k = 0; k < 4; ++k) h[k] = j + k < p.cols ? src[j + k] : 0;
+                q = make_uint2(h[0] | h[1] << 16, h[2] | h[3] << 16);
+            }
+            *reinterpret_cast<uint2*>(dst + j) = q;
+        }
     }
 }
 
@@ -78,92 +98,131 @@ __device__ __forceinline__ float tf32_nearest(float x) {
     return __uint_as_float((r & 0x7F800000u) == 0x7F800000u ? u & 0xFFFFE000u : r);
 }
 
-__global__ void __launch_bounds__(256) pack_split_kernel(const PackParams p) {
-    const int64_t total = p.dst_rows * p.dst_cols;
-    const float* src = static_cast<const float*>(p.src);
-    float* dst = static_cast<float*>(p.dst);
-    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
-         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t i = e / p.dst_cols, j = e - i * p.dst_cols;
-        const bool live = i < p.rows && j < p.cols && (p.targets == nullptr || __ldg(p.targets + i) != kEmptyToken);
-        const float x = live ? src[i * p.src_ld + j] : 0.0f;
-        // An infinity or NaN stays whole in the leading part (inf - inf would make the rest NaN).
-        const bool finite = (__float_as_uint(x) & 0x7F800000u) != 0x7F800000u;
-        const float hi = finite ? tf32_nearest(x) : x;
-        const float lo = finite ? tf32_nearest(x - hi) : 0.0f;
+__global__ void __launch_bounds__(256) pack_split_kernel(const PackParams p, int vec) {
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; i < p.dst_rows;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        const bool live = i < p.rows && has_target(p.targets, i);
+        const float* src = static_cast<const float*>(p.src) + i * p.src_ld;
+        float* dst = static_cast<float*>(p.dst) + i * p.dst_ld;
+        for (int64_t j = 4 * threadIdx.x; j < p.dst_cols; j += 4 * blockDim.x) {
+            float x[4] = {0.0f, 0.0f, 0.0f, 0.0f}, hi[4], lo[4];
+            if (live && vec && j + 4 <= p.cols) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(src + j));
+                x[0] = q.x; x[1] = q.y; x[2] = q.z; x[3] = q.w;
+            } else if (live) {
 #pragma unroll
-        for (int k = 0; k < 3; ++k) dst[p.plane[k] + i * p.dst_ld + j] = (p.low >> k) & 1 ? lo : hi;
+                for (int k = 0; k < 4; ++k) x[k] = j + k < p.cols ? src[j + k] : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 4; ++k) {
+                // An infinity or NaN stays whole in the leading part (inf - inf would make the rest NaN).
+                const bool finite = (__float_as_uint(x[k]) & 0x7F800000u) != 0x7F800000u;
+                hi[k] = finite ? tf32_nearest(x[k]) : x[k];
+                lo[k] = finite ? tf32_nearest(x[k] - hi[k]) : 0.0f;
+            }
+#pragma unroll
+            for (int k = 0; k < 3; ++k)
+                *reinterpret_cast<float4*>(dst + p.plane[k] + j) =
+                    (p.low >> k) & 1 ? make_float4(lo[0], lo[1], lo[2], lo[3]) : make_float4(hi[0], hi[1], hi[2], hi[3]);
+        }
     }
 }
 
-// out[i, j] (+)= ws[i, j] for i < rows, j < cols.
+// out[i, j] (+)= ws[i, j] for i < rows, j < cols; the workspace's rows are multiples of 4 elements.
 __global__ void __launch_bounds__(256) store_kernel(const float* ws, int64_t ws_ld, void* out, int out_bf16,
-                                                    int64_t out_ld, int64_t rows, int64_t cols, int accumulate) {
-    const int64_t total = rows * cols;
-    for (int64_t e = blockIdx.x * static_cast<int64_t>(blockDim.x) + threadIdx.x; e < total;
-         e += static_cast<int64_t>(gridDim.x) * blockDim.x) {
-        const int64_t i = e / cols, j = e - i * cols;
-        const float v = ws[i * ws_ld + j];
-        if (out_bf16) {
-            static_cast<uint16_t*>(out)[i * out_ld + j] = bf16_bits(v);
-        } else {
-            float* o = static_cast<float*>(out) + i * out_ld + j;
-            *o = accumulate ? *o + v : v;
+                                                    int64_t out_ld, int64_t rows, int64_t cols, int accumulate, int vec) {
+    allow_next_kernel();
+    wait_for_previous_kernel();
+    for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; i < rows;
+         i += static_cast<int64_t>(gridDim.x) * blockDim.y) {
+        const float* src = ws + i * ws_ld;
+        for (int64_t j = 4 * threadIdx.x; j < cols; j += 4 * blockDim.x) {
+            const float4 q = *reinterpret_cast<const float4*>(src + j);
+            const float v[4] = {q.x, q.y, q.z, q.w};
+            const int n = static_cast<int>(min(static_cast<int64_t>(4), cols - j));
+            if (out_bf16) {
+                uint16_t* dst = static_cast<uint16_t*>(out) + i * out_ld + j;
+                if (vec && n == 4)
+                    *reinterpret_cast<uint2*>(dst) = make_uint2(bf16_bits(v[0]) | static_cast<uint32_t>(bf16_bits(v[1])) << 16,
+                                                                bf16_bits(v[2]) | static_cast<uint32_t>(bf16_bits(v[3])) << 16);
+                else
+                    for (int k = 0; k < n; ++k) dst[k] = bf16_bits(v[k]);
+            } else {
+                float* dst = static_cast<float*>(out) + i * out_ld + j;
+                if (vec && n == 4 && !accumulate)
+                    *reinterpret_cast<float4*>(dst) = q;
+                else
+                    for (int k = 0; k < n; ++k) dst[k] = accumulate ? dst[k] + v[k] : v[k];
+            }
         }
     }
 }
 
 constexpr int kCombineRows = 32, kCombineLanes = 32;
 
-// Joins the (maximum, sum) pairs of each row: the block's 32 rows lie along the threads of a warp (coalesced
-// reads), its 32 warps take every 32nd pair, and their results are joined in warp order, so the result does not depend
-// on scheduling. Writes the row's loss and, for pass 2, (log2 e maximum, log2 sum), with a maximum of +inf in a row
-// without a target (every exponential is then 0) and NaN for a target that is no class. A grid of one block
-// also writes the sum of the losses.
+// Joins a (maximum, sum) pair into another.
+__device__ __forceinline__ void join(float2& a, float2 b) {
+    const float inf = __int_as_float(0x7f800000);
+    const float next = fmaxf(a.x, b.x);
+    const float base = next == -inf ? 0.0f : __fmul_rn(next, kLog2e);
+    a.y = a.y * exp2f(__fmul_rn(a.x, kLog2e) - base) + b.y * exp2f(__fmul_rn(b.x, kLog2e) - base);
+    a.x = next;
+}
+
+// Joins the (maximum, sum) pairs of each row: the block's 32 rows lie along the threads of a warp (coalesced reads), its
+// 32 warps take every 32nd pair; then a warp for each row joins the 32 results in a fixed tree, so the result does not
+// depend on scheduling. Writes the row's loss and, for pass 2, (log2 e maximum, log2 sum), with a maximum of +inf in a row
+// without a target (every exponential is then 0) and NaN for a target that is no class. A grid of one block also writes
+// the sum of the losses.
 __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     combine_kernel(const float2* partials, int64_t pairs, int64_t rows, const uint32_t* targets, uint64_t classes,
                    const float* target_logit, float* losses, float2* row_stats, float* loss_sum) {
-    __shared__ float2 part[kCombineLanes][kCombineRows];
+    __shared__ float2 part[kCombineLanes][kCombineRows + 1];
+    __shared__ float row_loss[kCombineRows];
+    allow_next_kernel();
+    wait_for_previous_kernel();
     const int r = threadIdx.x & 31, w = threadIdx.x >> 5;
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
     const float inf = __int_as_float(0x7f800000);
-    float m = -inf, s = 0.0f;
-    auto join = [&](float2 v) {
-        const float next = fmaxf(m, v.x);
-        const float base = next == -inf ? 0.0f : __fmul_rn(next, kLog2e);
-        s = s * exp2f(__fmul_rn(m, kLog2e) - base) + v.y * exp2f(__fmul_rn(v.x, kLog2e) - base);
-        m = next;
-    };
-    if (row < rows) {
+    float2 v = make_float2(-inf, 0.0f);
+    const int64_t read_row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
+    if (read_row < rows) {
 #pragma unroll 4
-        for (int64_t k = w; k < pairs; k += kCombineLanes) join(__ldg(partials + k * rows + row));
+        for (int64_t k = w; k < pairs; k += kCombineLanes) join(v, partials[k * rows + read_row]);
     }
-    part[w][r] = make_float2(m, s);
+    part[w][r] = v;
     __syncthreads();
-    if (w != 0) return;
-    m = -inf;
-    s = 0.0f;
-    for (int k = 0; k < kCombineLanes; ++k) join(part[k][r]);
+    v = part[r][w];
+#pragma unroll
+    for (int d = 16; d > 0; d >>= 1) {
+        const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d));
+        join(v, other);
+    }
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + w;
     float loss = 0.0f;
-    if (row < rows) {
+    if (r == 0 && row < rows) {
         const uint32_t t = targets[row];
         const float nan = __int_as_float(0x7fc00000);
-        if (t != kEmptyToken) loss = t < classes ? (m - target_logit[row]) + logf(s) : nan;
+        if (t != kEmptyToken) loss = t < classes ? (v.x - target_logit[row]) + logf(v.y) : nan;
         losses[row] = loss;
         if (row_stats != nullptr)
             row_stats[row] = t == kEmptyToken ? make_float2(inf, 0.0f)
-                                              : make_float2(t < classes ? __fmul_rn(m, kLog2e) : nan, log2f(s));
+                                              : make_float2(t < classes ? __fmul_rn(v.x, kLog2e) : nan, log2f(v.y));
     }
-    if (loss_sum != nullptr && gridDim.x == 1) {
+    if (loss_sum == nullptr || gridDim.x > 1) return;
+    if (r == 0) row_loss[w] = loss;
+    __syncthreads();
+    if (w != 0) return;
+    loss = row_loss[r];
 #pragma unroll
-        for (int d = 16; d > 0; d >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, d);
-        if (r == 0) *loss_sum = loss;
-    }
+    for (int d = 16; d > 0; d >>= 1) loss += __shfl_xor_sync(0xffffffffu, loss, d);
+    if (r == 0) *loss_sum = loss;
 }
 
 // The sum of the losses of more than 32 rows: one block, each thread every 1024th row, then a tree.
 __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* losses, int64_t rows, float* loss_sum) {
     __shared__ double part[32];
+    allow_next_kernel();
+    wait_for_previous_kernel();
     double s = 0.0;
     for (int64_t i = threadIdx.x; i < rows; i += 1024) s += static_cast<double>(losses[i]);
 #pragma unroll
@@ -195,7 +254,7 @@ struct Layout {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
-Layout layout_of(const snb_vocabulary_loss_args& a) {
+Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     Layout l{};
     l.f32 = a.type == SNB_TYPE_F32;
     l.gradients = a.hidden_grad != nullptr || a.weight_grad != nullptr;
@@ -208,14 +267,30 @@ Layout layout_of(const snb_vocabulary_loss_args& a) {
     // (The hidden gradient's product has `seg` columns: those past the width must be zeros of a packed weight.)
     l.pack_weight = l.f32 || !aligned16(a.weight) || a.weight_stride % per16 != 0 ||
                     (a.hidden_grad != nullptr && a.width != l.seg);
-    // A piece is as long as the bound allows for P [rows, piece] and for the packed weight, in whole tiles.
-    uint64_t piece = round_up(a.classes, 256);
-    auto bound = [&](uint64_t bytes_a_class) {
-        piece = std::min(piece, std::max<uint64_t>(256, kPieceBytes / std::max<uint64_t>(1, bytes_a_class) / 256 * 256));
+    // A piece is as long as the bounds allow for P [rows, piece] and for the packed weight, in whole tiles: long pieces
+    // make long sums for the hidden gradient and few additions into it. Between half that length and all of it, the one is
+    // taken whose weight gradient fills the last round of CTA pairs best (measured at 16,384 x 768 x 131,072: pieces of
+    // 8,192 classes, 96 tiles on 74 pairs, 12.3 ms; of 12,544, 147 tiles, 10.7 ms; of 16,384, 192 tiles, 10.5 ms).
+    uint64_t tiles = (a.classes + 255) / 256;
+    auto bound = [&](uint64_t bytes, uint64_t bytes_a_class) {
+        tiles = std::min(tiles, std::max<uint64_t>(1, bytes / std::max<uint64_t>(1, bytes_a_class) / 256));
     };
-    if (l.gradients) bound(a.rows * (l.f32 ? 8 : 2));
-    if (l.pack_weight) bound(l.f32 ? 12 * l.seg : 2 * l.seg);
-    l.piece = std::min(piece, a.classes);
+    if (l.gradients) bound(kPieceBytes, a.rows * (l.f32 ? 8 : 2));
+    if (l.pack_weight) bound(kWeightBytes, l.f32 ? 12 * l.seg : 2 * l.seg);
+    if (tiles * 256 < a.classes && a.weight_grad != nullptr) {
+        const uint64_t across = (a.width + 255) / 256, pairs = static_cast<uint64_t>(std::max(1, sms / 2));
+        uint64_t best = tiles;
+        double best_fill = 0.0;
+        for (uint64_t t = tiles; t >= std::max<uint64_t>(1, tiles / 2) && t > 0; --t) {
+            const double fill = static_cast<double>(t * across) / static_cast<double>(round_up(t * across, pairs));
+            if (fill > best_fill + 1e-9) {
+                best = t;
+                best_fill = fill;
+            }
+        }
+        tiles = best;
+    }
+    l.piece = std::min(tiles * 256, a.classes);
     l.pieces = (a.classes + l.piece - 1) / l.piece;
     const uint64_t piece_ld = round_up(l.piece, 8);
     l.hidden_ld = l.pack_hidden ? (l.f32 ? 3 * l.seg : l.seg) : a.hidden_stride;
@@ -243,6 +318,21 @@ Layout layout_of(const snb_vocabulary_loss_args& a) {
     return l;
 }
 
+// Launches a kernel that waits for the one before it by itself.
+template <typename... KArgs, typename... Args>
+void launch_early(void (*kernel)(KArgs...), unsigned grid, dim3 threads, cudaStream_t stream, Args... args) {
+    cudaLaunchConfig_t cfg{};
+    cfg.gridDim = dim3(grid);
+    cfg.blockDim = threads;
+    cfg.stream = stream;
+    cudaLaunchAttribute attr[1];
+    attr[0].id = cudaLaunchAttributeProgrammaticStreamSerialization;
+    attr[0].val.programmaticStreamSerializationAllowed = 1;
+    cfg.attrs = attr;
+    cfg.numAttrs = 1;
+    cudaLaunchKernelEx(&cfg, kernel, static_cast<KArgs>(args)...);
+}
+
 int launched(const char* what, std::string* err) {
     const cudaError_t e = cudaGetLastError();
     if (e == cudaSuccess) return SNB_OK;
@@ -250,8 +340,15 @@ int launched(const char* what, std::string* err) {
     return SNB_ERR_CUDA;
 }
 
-unsigned flat_grid(uint64_t elements, int sms) {
-    return static_cast<unsigned>(std::max<uint64_t>(1, std::min<uint64_t>((elements + 255) / 256, 8ull * sms)));
+// Threads and blocks of the elementwise kernels for rows x cols: as many threads along a row as have 4 columns, a power of
+// two, and enough blocks to fill the device eight times over at most.
+dim3 row_threads(uint64_t cols) {
+    unsigned x = 1;
+    while (x < 256 && 4ull * x < cols) x *= 2;
+    return dim3(x, 256 / x);
+}
+unsigned row_blocks(uint64_t rows, dim3 threads, int sms) {
+    return static_cast<unsigned>(std::max<uint64_t>(1, std::min<uint64_t>((rows + threads.y - 1) / threads.y, 8ull * sms)));
 }
 
 // One call's stream, arguments and choices, and the products it issues.
@@ -286,9 +383,11 @@ struct Call {
         p.targets = targets;
         for (int k = 0; k < 3; ++k) p.plane[k] = static_cast<int64_t>(k * plane);
         p.low = low;
-        const unsigned grid = flat_grid(dst_rows * dst_cols, sms);
-        if (l.f32) pack_split_kernel<<<grid, 256, 0, stream>>>(p);
-        else pack_bf16_kernel<<<grid, 256, 0, stream>>>(p);
+        const dim3 threads = row_threads(dst_cols);
+        const unsigned grid = row_blocks(dst_rows, threads, sms);
+        const int vec = reinterpret_cast<uintptr_t>(src) % (4 * l.elem) == 0 && src_ld % 4 == 0;
+        if (l.f32) pack_split_kernel<<<grid, threads, 0, stream>>>(p, vec);
+        else pack_bf16_kernel<<<grid, threads, 0, stream>>>(p, vec);
         return launched("vocabulary loss pack kernel launch", err);
     }
 
@@ -343,9 +442,10 @@ struct Call {
         return v;
     }
 
-    // C [rows, cols] (dense) (+)= grad_scale * A B; for f32 the three products of the split operands.
+    // C [rows, cols] (dense) (+)= grad_scale * A B; for f32 the three products of the split operands. c_ld: rows of C that
+    // far apart, on the tensor cores or (`tensor_only` false) not at all.
     int product(uint64_t rows, uint64_t cols, uint64_t inner, Part A, snb_operand left, Part B, snb_operand right,
-                void* C, int c_type, bool accumulate) const {
+                void* C, int c_type, bool accumulate, uint64_t c_ld = 0, bool* tensor_only = nullptr) const {
         GemmRequest r{};
         r.p.rows = rows;
         r.p.cols = cols;
@@ -362,28 +462,47 @@ struct Call {
         r.aux_type = c_type;
         r.deterministic = deterministic;
         r.sm_budget = sm_budget;
+        r.c_ld = c_ld;
         auto issue = [&]() {
             bool tensor = false;
             int path = 0;
             int rc = tc_gemm_try(stream, r, &tensor, &path, err);
-            if (rc == SNB_OK && !tensor) rc = simt_gemm(stream, r, err);
+            if (tensor_only != nullptr) *tensor_only = tensor;
+            else if (rc == SNB_OK && !tensor) rc = simt_gemm(stream, r, err);
             r.p.accumulate = 1;
             return rc;
         };
-        r.A = l.f32 ? A.low : A.lead;
+        r.A = A.lead;
+        r.B = B.lead;
+        if (!l.f32) return issue();
+        if (!deterministic) {
+            // All three products in one launch, where the small ones share the splits of the large one.
+            auto lower = [](const Part& x) { return x.low < x.lead ? x.low : x.lead; };
+            auto apart = [](const Part& x) {
+                const auto lead = static_cast<const float*>(x.lead), low = static_cast<const float*>(x.low);
+                return static_cast<uint64_t>(lead < low ? low - lead : lead - low);
+            };
+            r.A = lower(A);
+            r.B = lower(B);
+            r.split_inner = kSumLength;
+            r.a_plane_stride = apart(A);
+            r.b_plane_stride = apart(B);
+            r.a_low = A.low < A.lead ? 0 : 1;
+            r.b_low = B.low < B.lead ? 0 : 1;
+            bool tensor = false;
+            int path = 0;
+            const int rc = tc_gemm_try(stream, r, &tensor, &path, err);
+            if (rc != SNB_OK || tensor) return rc;
+            r.split_inner = 0;
+        }
+        // One product after the other, the one of the leading parts in pieces of K: the deterministic order, and the way for
+        // layouts that the tensor cores cannot read.
+        r.A = A.low;
         r.B = B.lead;
         int rc = issue();
-        if (rc != SNB_OK || !l.f32) return rc;
         r.A = A.lead;
         r.B = B.low;
-        if ((rc = issue()) != SNB_OK) return rc;
-        // The leading parts' product in sums of kSumLength, which meet in f32 additions that round to nearest: as splits
-        // of one launch, or in the deterministic mode as one launch after the other.
-        r.B = B.lead;
-        if (!deterministic) {
-            r.max_split_inner = kSumLength;
-            return issue();
-        }
+        if (rc == SNB_OK) rc = issue();
         for (uint64_t k = 0; k < inner && rc == SNB_OK; k += kSumLength) {
             r.p.inner = std::min(kSumLength, inner - k);
             r.A = static_cast<const float*>(A.lead) + k * left.col_stride;
@@ -395,9 +514,10 @@ struct Call {
 
     int store(const void* ws, uint64_t ws_ld, void* out, int out_type, uint64_t out_ld, uint64_t rows, uint64_t cols,
               bool accumulate) const {
-        store_kernel<<<flat_grid(rows * cols, sms), 256, 0, stream>>>(
-            static_cast<const float*>(ws), static_cast<int64_t>(ws_ld), out, out_type == SNB_TYPE_BF16,
-            static_cast<int64_t>(out_ld), static_cast<int64_t>(rows), static_cast<int64_t>(cols), accumulate);
+        const dim3 threads = row_threads(cols);
+        const int vec = reinterpret_cast<uintptr_t>(out) % (out_type == SNB_TYPE_BF16 ? 8 : 16) == 0 && out_ld % 4 == 0;
+        launch_early(store_kernel, row_blocks(rows, threads, sms), threads, stream, static_cast<const float*>(ws), ws_ld, out,
+                     out_type == SNB_TYPE_BF16, out_ld, rows, cols, accumulate, vec);
         return launched("vocabulary loss store kernel launch", err);
     }
 
@@ -406,6 +526,12 @@ struct Call {
         const snb_operand left{l.grad_ld, 1, 0};
         const snb_operand right = a.weight_transposed ? snb_operand{l.weight_ld, 1, 0} : snb_operand{1, l.weight_ld, 0};
         return product(a.rows, l.seg, n, grad_part(), left, weight_part(w), right, at(l.dh_at), SNB_TYPE_F32, v0 > 0);
+    }
+
+    // Whether an output's tiles, unsplit, keep three fifths of the CTA pairs' rounds busy.
+    bool fills(uint64_t rows, uint64_t cols) const {
+        const uint64_t tiles = (rows + 255) / 256 * ((cols + 255) / 256), pairs = static_cast<uint64_t>(std::max(1, sms / 2));
+        return tiles * 10 >= round_up(tiles, pairs) * 6;
     }
 
     // dW (+)= P^T H of one piece (or its transpose, for a [width, classes] weight).
@@ -418,14 +544,19 @@ struct Call {
             // The rows of the piece are contiguous in the gradient: written there unless a row is no multiple of 16
             // bytes, or a bf16 gradient has so few tiles that its sums are better split (which needs f32).
             const bool dense = a.width * es % 16 == 0 && aligned16(out);
-            const uint64_t tiles = (n + 255) / 256 * ((a.width + 255) / 256), pairs = static_cast<uint64_t>(sms / 2);
-            const bool fills = tiles * 10 >= (tiles + pairs - 1) / pairs * pairs * 6;
-            if (dense && (a.weight_grad_type == SNB_TYPE_F32 || fills))
+            if (dense && (a.weight_grad_type == SNB_TYPE_F32 || fills(n, a.width)))
                 return product(n, a.width, a.rows, grad_part(), p_t, hidden_part(), h, out, a.weight_grad_type,
                                a.accumulate != 0);
             rc = product(n, l.seg, a.rows, grad_part(), p_t, hidden_part(), h, at(l.dw_at), SNB_TYPE_F32, false);
             return rc != SNB_OK ? rc : store(at(l.dw_at), l.wgrad_ld, out, a.weight_grad_type, a.width, n, a.width,
                                              a.accumulate != 0);
+        }
+        // The gradient's rows are strided here: written there under the same conditions, if no sums are split.
+        if (a.classes * es % 16 == 0 && aligned16(out) && !l.f32 && a.accumulate == 0 && fills(a.width, n)) {
+            bool tensor = false;
+            rc = product(a.width, n, a.rows, hidden_part(), h_t, grad_part(), p_n, out, a.weight_grad_type, false, a.classes,
+                         &tensor);
+            if (rc != SNB_OK || tensor) return rc;
         }
         // Rows of round_up(n, 8) columns: those past n come from P's padding, are never stored, and touch no others.
         const uint64_t cols = round_up(n, 8);
@@ -451,14 +582,13 @@ struct Call {
             if ((rc = tc_vocab_product(stream, logits(v0, n, w), err)) != SNB_OK) return rc;
         }
         const uint64_t blocks = (a.rows + kCombineRows - 1) / kCombineRows;
-        combine_kernel<<<static_cast<unsigned>(blocks), kCombineRows * kCombineLanes, 0, stream>>>(
-            static_cast<const float2*>(at(l.partials_at)),
-            static_cast<int64_t>((a.classes + kHalfTile - 1) / kHalfTile), static_cast<int64_t>(a.rows), a.targets,
-            a.classes, static_cast<const float*>(at(l.target_at)), a.losses,
-            l.gradients ? static_cast<float2*>(at(l.stats_at)) : nullptr, a.loss_sum);
+        launch_early(combine_kernel, static_cast<unsigned>(blocks), kCombineRows * kCombineLanes, stream,
+                     static_cast<const float2*>(at(l.partials_at)), (a.classes + kHalfTile - 1) / kHalfTile, a.rows, a.targets,
+                     a.classes, static_cast<const float*>(at(l.target_at)), a.losses,
+                     l.gradients ? static_cast<float2*>(at(l.stats_at)) : nullptr, a.loss_sum);
         if ((rc = launched("combine_kernel launch", err)) != SNB_OK) return rc;
         if (a.loss_sum != nullptr && blocks > 1) {
-            loss_sum_kernel<<<1, 1024, 0, stream>>>(a.losses, static_cast<int64_t>(a.rows), a.loss_sum);
+            launch_early(loss_sum_kernel, 1, 1024, stream, a.losses, a.rows, a.loss_sum);
             if ((rc = launched("loss_sum_kernel launch", err)) != SNB_OK) return rc;
         }
         if (!l.gradients) return SNB_OK;
@@ -482,9 +612,11 @@ struct Call {
 
 }  // namespace
 
-int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std::string*) {
-    *bytes = layout_of(a).bytes;
-    return SNB_OK;
+int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std::string* err) {
+    DeviceInfo dev{};
+    const int rc = a.rows == 0 ? SNB_OK : current_device_info(&dev, err);
+    if (rc == SNB_OK) *bytes = layout_of(a, dev.sm_count).bytes;
+    return rc;
 }
 
 int vocab_loss_launch(cudaStream_t stream, const snb_vocabulary_loss_args& a, bool deterministic, int sm_budget,
@@ -503,7 +635,7 @@ int vocab_loss_launch(cudaStream_t stream, const snb_vocabulary_loss_args& a, bo
     const int rc = current_device_info(&dev, err);
     if (rc != SNB_OK) return rc;
     const uintptr_t base = (reinterpret_cast<uintptr_t>(a.workspace) + 255) & ~uintptr_t(255);
-    return Call{stream, a, layout_of(a), deterministic, sm_budget, dev.sm_count, reinterpret_cast<uint8_t*>(base), err}.run();
+    return Call{stream, a, layout_of(a, dev.sm_count), deterministic, sm_budget, dev.sm_count, reinterpret_cast<uint8_t*>(base), err}.run();
 }
 
 }  // namespace snb
