@@ -603,8 +603,10 @@ int snb_vocabulary_cross_entropy(void* stream, const snb_vocabulary_loss_args* a
     rc = vocab_loss_launch(static_cast<cudaStream_t>(stream), *args,
                            t_deterministic || (args->flags & SNB_GEMM_DETERMINISTIC) != 0, t_sm_budget, &err);
     if (rc != SNB_OK) return fail(rc, err);
-    t_last_path = args->rows == 0 ? SNB_PATH_EMPTY
-                                  : (args->rows > 128 ? SNB_PATH_TENSOR_CORE_PAIR : SNB_PATH_TENSOR_CORE);
+    t_last_path = args->rows == 0                ? SNB_PATH_EMPTY
+                 : vocab_loss_few_rows(*args) ? SNB_PATH_SIMT
+                 : args->rows > 128           ? SNB_PATH_TENSOR_CORE_PAIR
+                                              : SNB_PATH_TENSOR_CORE;
     return SNB_OK;
 }
 

@@ -138,6 +138,7 @@ struct VocabProduct {
 int tc_vocab_product(cudaStream_t stream, const VocabProduct& v, std::string* err);
 
 // Softmax cross entropy over a vocabulary in pieces (vocab_loss.cu).
+bool vocab_loss_few_rows(const snb_vocabulary_loss_args& a);  // whether the CUDA cores compute the logits
 int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std::string* err);
 int vocab_loss_launch(cudaStream_t stream, const snb_vocabulary_loss_args& a, bool deterministic, int sm_budget,
                       std::string* err);

@@ -13,6 +13,7 @@
 #include <cuda_runtime.h>
 
 #include <algorithm>
+#include <atomic>
 #include <cmath>
 #include <cstdint>
 #include <string>
@@ -681,11 +682,18 @@ int launched(const char* what, std::string* err) {
 }
 
 // Launches `kernel` with a ring of its own size. Above 48 KB together with the kernel's static shared memory (4 KB at
-// most) that has to be allowed first, a setting of the kernel on the current device that is cheap to repeat.
-template <typename Kernel>
-void launch_ring(Kernel kernel, unsigned grid, int threads, int64_t smem, cudaStream_t s, const NormParams& p) {
-    if (smem > (44 << 10))
-        cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+// most) that has to be allowed first, a setting of the kernel on its device that is made again when either changes.
+template <auto kernel>
+void launch_ring(unsigned grid, int threads, int64_t smem, cudaStream_t s, const NormParams& p) {
+    static std::atomic<int64_t> allowed{-1};  // device << 32 | bytes
+    if (smem > (44 << 10)) {
+        int dev = 0;
+        cudaGetDevice(&dev);
+        const int64_t want = static_cast<int64_t>(dev) << 32 | smem;
+        if (allowed.load(std::memory_order_relaxed) != want &&
+            cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess)
+            allowed.store(want, std::memory_order_relaxed);
+    }
     kernel<<<grid, threads, static_cast<size_t>(smem), s>>>(p);
 }
 
@@ -697,8 +705,8 @@ void forward_typed(NormParams p, int sms, cudaStream_t s) {
     const int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
     const int64_t blocks = T == 32 ? (p.rows + kWarpsPerBlock - 1) / kWarpsPerBlock : p.rows;
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, (T == 1024 ? 1ll : T == 256 ? 4ll : 2ll) * sms));
-    if (p.x_bf16) launch_ring(layer_norm_kernel<T, NE, G, true>, grid, threads, smem, s, p);
-    else launch_ring(layer_norm_kernel<T, NE, G, false>, grid, threads, smem, s, p);
+    if (p.x_bf16) launch_ring<layer_norm_kernel<T, NE, G, true>>(grid, threads, smem, s, p);
+    else launch_ring<layer_norm_kernel<T, NE, G, false>>(grid, threads, smem, s, p);
 }
 
 // group: the columns of 16 bytes of the call's widest type, or 1 where its rows do not allow 16-byte accesses.
@@ -716,13 +724,13 @@ void backward_typed(NormParams p, unsigned grid, cudaStream_t s) {
     p.depth = depth_of({T, NE}, slot);
     int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
     if (T == 32) smem = std::max<int64_t>(smem, 2 * kWarpsPerBlock * p.cols * static_cast<int64_t>(sizeof(float)));
-    if (p.x_bf16 && p.dy_bf16) launch_ring(layer_norm_backward_kernel<T, NE, G, true, true>, grid, threads, smem, s, p);
+    if (p.x_bf16 && p.dy_bf16) launch_ring<layer_norm_backward_kernel<T, NE, G, true, true>>(grid, threads, smem, s, p);
     else if (p.x_bf16) {
-        if constexpr (G != 8) launch_ring(layer_norm_backward_kernel<T, NE, G, true, false>, grid, threads, smem, s, p);
+        if constexpr (G != 8) launch_ring<layer_norm_backward_kernel<T, NE, G, true, false>>(grid, threads, smem, s, p);
     } else if (p.dy_bf16) {
-        if constexpr (G != 8) launch_ring(layer_norm_backward_kernel<T, NE, G, false, true>, grid, threads, smem, s, p);
+        if constexpr (G != 8) launch_ring<layer_norm_backward_kernel<T, NE, G, false, true>>(grid, threads, smem, s, p);
     } else {
-        if constexpr (G != 8) launch_ring(layer_norm_backward_kernel<T, NE, G, false, false>, grid, threads, smem, s, p);
+        if constexpr (G != 8) launch_ring<layer_norm_backward_kernel<T, NE, G, false, false>>(grid, threads, smem, s, p);
     }
 }
 

@@ -218,6 +218,226 @@ __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     if (r == 0) *loss_sum = loss;
 }
 
+// The loss alone of a few rows where the tensor cores could not read the weight as it lies (see few_rows): up to four rows
+// in one pass over the weight, which is what bounds it, on the CUDA cores. Logits are f32 sums; each thread block leaves one
+// (maximum, sum) pair for each row.
+constexpr int kFewThreads = 256;
+
+struct FewParams {
+    const void* hidden;
+    int64_t hidden_ld;
+    const void* weight;
+    int64_t weight_ld;
+    int32_t rows, all_rows, width;  // of this launch (1 to 4) and of the call
+    int64_t classes;
+    const uint32_t* targets;
+    float2* partials;               // [blocks, all_rows], from this launch's first row on
+    float* target_logit;
+    int32_t vec;  // 16-byte accesses to the weight's rows
+};
+
+__device__ __forceinline__ float element_of(const float* p, int64_t i) { return p[i]; }
+__device__ __forceinline__ float element_of(const uint16_t* p, int64_t i) {
+    return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
+}
+
+// 16 bytes of a row as floats: 4 of f32, 8 of bf16.
+__device__ __forceinline__ void unpack(uint4 q, float (&v)[4]) {
+    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
+}
+__device__ __forceinline__ void unpack(uint4 q, float (&v)[8]) {
+    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
+#pragma unroll
+    for (int k = 0; k < 4; ++k) {
+        v[2 * k] = __uint_as_float(w[k] << 16);
+        v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
+    }
+}
+
+// The hidden rows as f32 in shared memory, [R, ld], zero past the call's rows. LANES: in the order in which few_rows_kernel
+// reads bf16 weights, where a lane has 8 consecutive elements of each 256: the first halves of all lanes, then the second.
+template <int R, bool LANES, typename E>
+__device__ __forceinline__ void stage_hidden(const FewParams& p, float* h, int ld) {
+    for (int k = threadIdx.x; k < p.width; k += kFewThreads) {
+        const int at = LANES ? (k & ~255) + ((k & 4) << 5) + ((k & 0xF8) >> 1) + (k & 3) : k;
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+            h[r * ld + at] = r < p.rows ? element_of(static_cast<const E*>(p.hidden), r * p.hidden_ld + k) : 0.0f;
+    }
+    __syncthreads();
+}
+
+// Takes the logits z[0 .. n) of the classes from v on into a row's statistics.
+template <int N>
+__device__ __forceinline__ void take_logits(const FewParams& p, int r, int64_t v, const float (&z)[N], int n, float2& stats) {
+    const float inf = __int_as_float(0x7f800000);
+    float next = stats.x;
+#pragma unroll
+    for (int c = 0; c < N; ++c) next = c < n ? fmaxf(next, z[c]) : next;
+    const float base = next == -inf ? 0.0f : __fmul_rn(next, kLog2e);
+    float sum = stats.y * exp2f(__fmul_rn(stats.x, kLog2e) - base);
+#pragma unroll
+    for (int c = 0; c < N; ++c) sum += c < n ? exp2f(fmaf(z[c], kLog2e, -base)) : 0.0f;
+    stats = make_float2(next, sum);
+    const int64_t t = r < p.rows ? static_cast<int64_t>(__ldg(p.targets + r)) - v : -1;
+    if (t >= 0 && t < n) {
+#pragma unroll
+        for (int c = 0; c < N; ++c)
+            if (t == c) p.target_logit[r] = z[c];
+    }
+}
+
+// Leaves the block's pair of each row, joined from its warps' in a fixed order; every lane of a warp holds the warp's.
+template <int R>
+__device__ __forceinline__ void leave_pairs(const FewParams& p, const float2 (&stats)[R]) {
+    __shared__ float2 part[R][kFewThreads / 32];
+    if ((threadIdx.x & 31) == 0)
+#pragma unroll
+        for (int r = 0; r < R; ++r) part[r][threadIdx.x >> 5] = stats[r];
+    __syncthreads();
+    if (threadIdx.x < R && static_cast<int>(threadIdx.x) < p.rows) {
+        float2 v = part[threadIdx.x][0];
+        for (int w = 1; w < kFewThreads / 32; ++w) join(v, part[threadIdx.x][w]);
+        p.partials[static_cast<int64_t>(blockIdx.x) * p.all_rows + threadIdx.x] = v;
+    }
+}
+
+// Weight [classes, width]: a warp takes four classes at a time, its lanes 16 bytes of each row in turn.
+template <int R, typename E>
+__global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p) {
+    extern __shared__ __align__(16) float h[];
+    allow_next_kernel();
+    constexpr int PER = 16 / sizeof(E);
+    const int ld = (p.width + 255) & ~255;
+    if (PER == 8 && p.vec) stage_hidden<R, true, E>(p, h, ld);
+    else stage_hidden<R, false, E>(p, h, ld);
+    const int lane = threadIdx.x & 31;
+    const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kFewThreads / 32) + (threadIdx.x >> 5);
+    const int64_t warps = static_cast<int64_t>(gridDim.x) * (kFewThreads / 32);
+    const E* weight = static_cast<const E*>(p.weight);
+    float2 stats[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) stats[r] = make_float2(-__int_as_float(0x7f800000), 0.0f);
+    for (int64_t v0 = 4 * warp; v0 < p.classes; v0 += 4 * warps) {
+        const int n = static_cast<int>(min(static_cast<int64_t>(4), p.classes - v0));
+        float z[R][4];
+#pragma unroll
+        for (int r = 0; r < R; ++r) z[r][0] = z[r][1] = z[r][2] = z[r][3] = 0.0f;
+        const E* rows = weight + v0 * p.weight_ld;
+        if (p.vec) {
+#pragma unroll 3
+            for (int k = lane * PER; k < p.width; k += 32 * PER) {
+                uint4 q[4];
+#pragma unroll
+                for (int c = 0; c < 4; ++c)
+                    q[c] = c < n ? __ldg(reinterpret_cast<const uint4*>(rows + c * p.weight_ld + k)) : make_uint4(0, 0, 0, 0);
+#pragma unroll
+                for (int r = 0; r < R; ++r) {
+                    const float* hr = h + r * ld + (PER == 8 ? (k & ~255) + 4 * lane : k);
+                    float x[PER];
+#pragma unroll
+                    for (int e = 0; e < PER; e += 4) {
+                        const float4 f = *reinterpret_cast<const float4*>(hr + 32 * e);
+                        x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
+                    }
+#pragma unroll
+                    for (int c = 0; c < 4; ++c) {
+                        float w[PER];
+                        unpack(q[c], w);
+#pragma unroll
+                        for (int e = 0; e < PER; ++e) z[r][c] = fmaf(w[e], x[e], z[r][c]);
+                    }
+                }
+            }
+        } else {
+            for (int k = lane; k < p.width; k += 32)
+                for (int c = 0; c < n; ++c) {
+                    const float w = element_of(rows, c * p.weight_ld + k);
+#pragma unroll
+                    for (int r = 0; r < R; ++r) {
+                        const float sum = fmaf(w, h[r * ld + k], c == 0 ? z[r][0] : c == 1 ? z[r][1] : c == 2 ? z[r][2] : z[r][3]);
+                        if (c == 0) z[r][0] = sum;
+                        else if (c == 1) z[r][1] = sum;
+                        else if (c == 2) z[r][2] = sum;
+                        else z[r][3] = sum;
+                    }
+                }
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+#pragma unroll
+            for (int d = 16; d > 0; d >>= 1)
+#pragma unroll
+                for (int c = 0; c < 4; ++c) z[r][c] += __shfl_xor_sync(0xffffffffu, z[r][c], d);
+            take_logits(p, r, v0, z[r], n, stats[r]);
+        }
+    }
+    leave_pairs<R>(p, stats);
+}
+
+// Weight [width, classes]: a block takes 32 PER classes, a lane PER of them, its warps an eighth of the width each; their
+// sums meet in shared memory.
+template <int R, typename E>
+__global__ void __launch_bounds__(kFewThreads) few_rows_across_kernel(const FewParams p) {
+    extern __shared__ __align__(16) float h[];  // [R, width], then [8 warps, R, 32 PER] sums
+    allow_next_kernel();
+    stage_hidden<R, false, E>(p, h, p.width);
+    constexpr int PER = 16 / sizeof(E);
+    constexpr int WARPS = kFewThreads / 32;
+    float* sums = h + (R * p.width + 3) / 4 * 4;
+    const int lane = threadIdx.x & 31, w = threadIdx.x >> 5;
+    const int64_t v0 = static_cast<int64_t>(blockIdx.x) * 32 * PER;
+    const int64_t v = v0 + lane * PER;
+    const E* weight = static_cast<const E*>(p.weight);
+    float z[R][PER];
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) z[r][e] = 0.0f;
+    const int each = (p.width + WARPS - 1) / WARPS;
+    const int end = min(p.width, (w + 1) * each);
+    const bool whole = p.vec && v + PER <= p.classes;
+#pragma unroll 8
+    for (int k = w * each; k < end; ++k) {
+        const E* row = weight + static_cast<int64_t>(k) * p.weight_ld + v;
+        float x[PER];
+        if (whole) {
+            unpack(__ldg(reinterpret_cast<const uint4*>(row)), x);
+        } else {
+#pragma unroll
+            for (int e = 0; e < PER; ++e) x[e] = v + e < p.classes ? element_of(row, e) : 0.0f;
+        }
+#pragma unroll
+        for (int r = 0; r < R; ++r)
+#pragma unroll
+            for (int e = 0; e < PER; ++e) z[r][e] = fmaf(x[e], h[r * p.width + k], z[r][e]);
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int e = 0; e < PER; ++e) sums[(w * R + r) * 32 * PER + lane * PER + e] = z[r][e];
+    __syncthreads();
+    float2 stats[R];
+#pragma unroll
+    for (int r = 0; r < R; ++r) stats[r] = make_float2(-__int_as_float(0x7f800000), 0.0f);
+    for (int c = threadIdx.x; c < 32 * PER; c += kFewThreads) {
+#pragma unroll
+        for (int r = 0; r < R; ++r) {
+            float sum = 0.0f;
+#pragma unroll
+            for (int k = 0; k < WARPS; ++k) sum += sums[(k * R + r) * 32 * PER + c];
+            const float z1[1] = {sum};
+            if (v0 + c < p.classes) take_logits(p, r, v0 + c, z1, 1, stats[r]);
+        }
+    }
+#pragma unroll
+    for (int r = 0; r < R; ++r)
+#pragma unroll
+        for (int d = 16; d > 0; d >>= 1)
+            join(stats[r], make_float2(__shfl_xor_sync(0xffffffffu, stats[r].x, d), __shfl_xor_sync(0xffffffffu, stats[r].y, d)));
+    leave_pairs<R>(p, stats);
+}
+
 // The sum of the losses of more than 32 rows: one block, each thread every 1024th row, then a tree.
 __global__ void __launch_bounds__(1024) loss_sum_kernel(const float* losses, int64_t rows, float* loss_sum) {
     __shared__ double part[32];
@@ -241,7 +461,8 @@ uint64_t round_up(uint64_t n, uint64_t to) { return (n + to - 1) / to * to; }
 
 // The shapes and the workspace of one call. Offsets are from a 256-byte aligned base.
 struct Layout {
-    bool f32, gradients, pack_hidden, pack_weight;
+    bool f32, gradients, few, pack_hidden, pack_weight;
+    uint64_t few_blocks;    // thread blocks of the few rows' kernels
     uint64_t elem;          // bytes of an operand element
     uint64_t seg;           // width rounded up to 16 bytes: a packed row, or one of the three planes of an f32 row
     uint64_t k_logits;      // length of the logits' sums
@@ -254,6 +475,18 @@ struct Layout {
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
 
+// Whether the few rows' kernels take a call: the loss alone of hidden rows that fit into shared memory as f32 (64 KB for
+// four), where the tensor cores would need a packed copy of the weight first. Measured over 100,000 x 1,024 f32 (63 us at
+// the copy rate): 1 row 90 us, 4 rows 100 us, 5 rows by way of the split copy 634 us, so f32 goes up to 16 rows, four a
+// pass; over 512 x 50,021 bf16, whose rows lie off every boundary: 1 row 48 us, 4 rows 53 us, packed 62 us. A bf16 weight
+// that TMA can read stays with the tensor cores (32,000 x 768: 1 row 23 us here, 19 us there).
+bool few_rows(const snb_vocabulary_loss_args& a) {
+    const uint64_t per16 = a.type == SNB_TYPE_BF16 ? 8 : 4;
+    const bool readable = a.type == SNB_TYPE_BF16 && aligned16(a.weight) && a.weight_stride % per16 == 0;
+    return a.hidden_grad == nullptr && a.weight_grad == nullptr && !readable &&
+           a.rows <= (a.type == SNB_TYPE_BF16 ? 4 : 16) && a.width <= 4096;
+}
+
 Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     Layout l{};
     l.f32 = a.type == SNB_TYPE_F32;
@@ -261,12 +494,15 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.elem = l.f32 ? 4 : 2;
     const uint64_t per16 = 16 / l.elem;
     l.seg = round_up(a.width, per16);
+    l.few = few_rows(a);
+    l.few_blocks = a.weight_transposed ? std::min<uint64_t>((a.classes + 31) / 32, 4ull * sms)
+                                       : (a.classes + 32 * per16 - 1) / (32 * per16);
     l.k_logits = l.f32 ? 3 * l.seg : a.width;
     // The weight's gradient multiplies by the hidden rows without a target too: those have to be zero then.
-    l.pack_hidden = l.f32 || a.weight_grad != nullptr || !aligned16(a.hidden) || a.hidden_stride % per16 != 0;
+    l.pack_hidden = !l.few && (l.f32 || a.weight_grad != nullptr || !aligned16(a.hidden) || a.hidden_stride % per16 != 0);
     // (The hidden gradient's product has `seg` columns: those past the width must be zeros of a packed weight.)
-    l.pack_weight = l.f32 || !aligned16(a.weight) || a.weight_stride % per16 != 0 ||
-                    (a.hidden_grad != nullptr && a.width != l.seg);
+    l.pack_weight = !l.few && (l.f32 || !aligned16(a.weight) || a.weight_stride % per16 != 0 ||
+                               (a.hidden_grad != nullptr && a.width != l.seg));
     // A piece is as long as the bounds allow for P [rows, piece] and for the packed weight, in whole tiles: long pieces
     // make long sums for the hidden gradient and few additions into it. Between half that length and all of it, the one is
     // taken whose weight gradient fills the last round of CTA pairs best (measured at 16,384 x 768 x 131,072: pieces of
@@ -308,7 +544,7 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.hidden_at = take(l.pack_hidden ? a.rows * l.hidden_ld * l.elem : 0);
     l.weight_at = take(l.pack_weight ? (a.weight_transposed ? l.piece * l.weight_ld
                                                             : (l.f32 ? 3 : 1) * l.seg * l.weight_ld) * l.elem : 0);
-    l.partials_at = take((a.classes + kHalfTile - 1) / kHalfTile * a.rows * sizeof(float2));
+    l.partials_at = take((l.few ? l.few_blocks : (a.classes + kHalfTile - 1) / kHalfTile) * a.rows * sizeof(float2));
     l.target_at = take(a.rows * 4);
     l.stats_at = take(a.rows * sizeof(float2));
     l.p_at = take(l.gradients ? a.rows * l.grad_ld * (l.f32 ? 8 : 2) : 0);
@@ -565,6 +801,50 @@ struct Call {
                                          a.accumulate != 0);
     }
 
+    template <int R, typename E>
+    int few_typed(const FewParams& p) const {
+        int64_t smem = 4ll * R * (a.weight_transposed ? (p.width + 255) & ~255 : p.width);
+        if (!a.weight_transposed) smem = (smem + 15) / 16 * 16 + 4ll * kFewThreads * R * (16 / static_cast<int>(sizeof(E)));
+        const auto kernel = a.weight_transposed ? few_rows_kernel<R, E> : few_rows_across_kernel<R, E>;
+        if (smem > (44 << 10)) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+            if (e != cudaSuccess) {
+                *err = cuda_message("cudaFuncSetAttribute(few_rows_kernel)", e);
+                return SNB_ERR_CUDA;
+            }
+        }
+        kernel<<<static_cast<unsigned>(l.few_blocks), kFewThreads, static_cast<size_t>(smem), stream>>>(p);
+        return launched("few_rows_kernel launch", err);
+    }
+
+    int few() const {
+        FewParams p{};
+        p.hidden = a.hidden;
+        p.hidden_ld = static_cast<int64_t>(a.hidden_stride);
+        p.weight = a.weight;
+        p.weight_ld = static_cast<int64_t>(a.weight_stride);
+        p.all_rows = static_cast<int32_t>(a.rows);
+        p.width = static_cast<int32_t>(a.width);
+        p.classes = static_cast<int64_t>(a.classes);
+        p.targets = a.targets;
+        p.partials = static_cast<float2*>(at(l.partials_at));
+        p.target_logit = static_cast<float*>(at(l.target_at));
+        const uint64_t per16 = 16 / l.elem;
+        p.vec = aligned16(a.weight) && a.weight_stride % per16 == 0 && (!a.weight_transposed || a.width % per16 == 0);
+        for (uint64_t row = 0; row < a.rows; row += 4) {
+            p.rows = static_cast<int32_t>(std::min<uint64_t>(4, a.rows - row));
+            int rc;
+            if (l.f32) rc = p.rows == 1 ? few_typed<1, float>(p) : p.rows == 2 ? few_typed<2, float>(p) : few_typed<4, float>(p);
+            else rc = p.rows == 1 ? few_typed<1, uint16_t>(p) : p.rows == 2 ? few_typed<2, uint16_t>(p) : few_typed<4, uint16_t>(p);
+            if (rc != SNB_OK) return rc;
+            p.hidden = static_cast<const uint8_t*>(p.hidden) + 4 * a.hidden_stride * l.elem;
+            p.targets += 4;
+            p.partials += 4;
+            p.target_logit += 4;
+        }
+        return SNB_OK;
+    }
+
     int run() const {
         int rc = SNB_OK;
         constexpr int kLoHiHi = 1;
@@ -576,14 +856,15 @@ struct Call {
         // Pass 1: a weight that is read in place needs no pieces here.
         const uint64_t step = l.pack_weight ? l.piece : a.classes;
         const void* w = nullptr;
-        for (uint64_t v0 = 0; v0 < a.classes; v0 += step) {
+        if (l.few && (rc = few()) != SNB_OK) return rc;
+        for (uint64_t v0 = 0; v0 < a.classes && !l.few; v0 += step) {
             const uint64_t n = std::min(step, a.classes - v0);
             if ((rc = weight(v0, n, &w)) != SNB_OK) return rc;
             if ((rc = tc_vocab_product(stream, logits(v0, n, w), err)) != SNB_OK) return rc;
         }
         const uint64_t blocks = (a.rows + kCombineRows - 1) / kCombineRows;
         launch_early(combine_kernel, static_cast<unsigned>(blocks), kCombineRows * kCombineLanes, stream,
-                     static_cast<const float2*>(at(l.partials_at)), (a.classes + kHalfTile - 1) / kHalfTile, a.rows, a.targets,
+                     static_cast<const float2*>(at(l.partials_at)), l.few ? l.few_blocks : (a.classes + kHalfTile - 1) / kHalfTile, a.rows, a.targets,
                      a.classes, static_cast<const float*>(at(l.target_at)), a.losses,
                      l.gradients ? static_cast<float2*>(at(l.stats_at)) : nullptr, a.loss_sum);
         if ((rc = launched("combine_kernel launch", err)) != SNB_OK) return rc;
@@ -611,6 +892,8 @@ struct Call {
 };
 
 }  // namespace
+
+bool vocab_loss_few_rows(const snb_vocabulary_loss_args& a) { return few_rows(a); }
 
 int vocab_loss_workspace(const snb_vocabulary_loss_args& a, uint64_t* bytes, std::string* err) {
     DeviceInfo dev{};

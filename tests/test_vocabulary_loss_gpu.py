@@ -95,6 +95,22 @@ def test_losses_and_gradients(rows, width, classes, dtype, storage):
 
 
 @pytest.mark.parametrize("storage", list(Storage), ids=lambda s: s.name.lower())
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 16, 17])
+def test_the_loss_of_a_few_rows(rows, dtype, storage):
+    """Alone, over weights that the tensor cores can read and ones that they cannot (odd row lengths, off a boundary)."""
+    for width, classes, first in ((768, 3001, 0), (771, 2048, 0), (256, 40, 1), (5, 1, 0), (4096, 130, 0), (4100, 77, 3)):
+        hidden, weight, targets = _case(rows, width, classes, dtype, storage, seed=rows)
+        whole = torch.full((weight.shape[0], weight.shape[1] + first), float("nan"), device="cuda", dtype=dtype)
+        weight = whole[:, first:].copy_(weight)
+        losses_e, lse, size, *_ = _reference(hidden, weight, targets, storage, 1.0)
+        losses, total = _run(hidden, weight, targets, storage)
+        bound = (width / 8 + 8) * 2.0 ** -23 * 2 * size + 8 * 2.0 ** -23 * (lse.abs() + 1)
+        assert bool(((losses.double() - losses_e).abs() <= bound).all())
+        assert abs(total.double() - losses_e.sum()) <= bound.sum() + 2.0 ** -23 * losses_e.sum()
+
+
+@pytest.mark.parametrize("storage", list(Storage), ids=lambda s: s.name.lower())
 @pytest.mark.parametrize("rows,width,classes,dtype", [(8192, 40, 40001, BF16), (4096, 36, 20003, F32)])
 def test_a_vocabulary_of_several_pieces(rows, width, classes, dtype, storage):
     _check(*_case(rows, width, classes, dtype, storage, seed=5), storage)
