@@ -394,7 +394,7 @@ SNB_API int snb_codebook_cross_entropy(void* stream, const void* logits, int32_t
  * classes' weight rows w_v, z_v = h . w_v, losses[row] = log sum_v exp(z_v) - z_target, and with p = softmax(z) - onehot
  *   hidden_grad[row] = grad_scale * sum_v p_v w_v,   weight_grad[v] = grad_scale * sum_rows p_v h.
  * The vocabulary is taken in pieces: one pass over it for the rows' log-sum-exp, and for gradients a second one that
- * computes each piece's logits again, so the logits are never held. */
+ * computes each piece's logits again, so the logits are never held. Outputs overlap no input (hidden_grad may be hidden). */
 typedef struct snb_vocabulary_loss_args {
     uint64_t rows, width, classes;
     int32_t type;              /* SNB_TYPE_* of hidden and weight. bf16: bf16 tensor cores, p rounded to bf16 for the two

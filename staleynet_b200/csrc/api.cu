@@ -615,32 +615,29 @@ namespace {
 // One [rows, cols] tensor of a layer norm call; `what` names it in the message.
 int check_norm_tensor(const char* name, const char* what, const snb_layer_norm_args& a, const void* base, uint64_t len,
                       uint64_t stride, int32_t type, int too_small) {
-    const std::string at = std::string(name) + ": " + what;
-    if (type != SNB_TYPE_F32 && type != SNB_TYPE_BF16) return fail(SNB_ERR_INVALID_ARGUMENT, at + " has an unknown type");
-    if (stride < a.cols || stride > (1ull << 32)) return fail(SNB_ERR_INVALID_ARGUMENT, at + " stride out of range");
+    auto refuse = [&](int code, const char* why) { return fail(code, std::string(name) + ": " + what + why); };
+    if (type != SNB_TYPE_F32 && type != SNB_TYPE_BF16) return refuse(SNB_ERR_INVALID_ARGUMENT, " has an unknown type");
+    if (stride < a.cols || stride > (1ull << 32)) return refuse(SNB_ERR_INVALID_ARGUMENT, " stride out of range");
     if (a.rows == 0) return SNB_OK;
-    if (len < (a.rows - 1) * stride + a.cols) return fail(too_small, at + " too small");
-    if (base == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, at + " is null");
+    if (len < (a.rows - 1) * stride + a.cols) return refuse(too_small, " too small");
+    if (base == nullptr) return refuse(SNB_ERR_INVALID_ARGUMENT, " is null");
     if (reinterpret_cast<uintptr_t>(base) % (type == SNB_TYPE_BF16 ? 2 : 4) != 0)
-        return fail(SNB_ERR_INVALID_ARGUMENT, at + " is not aligned to its element");
+        return refuse(SNB_ERR_INVALID_ARGUMENT, " is not aligned to its element");
     return SNB_OK;
 }
 
 int check_layer_norm(const char* name, const snb_layer_norm_args* a) {
-    if (a == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, std::string(name) + ": args is null");
-    const std::string n(name);
+    auto refuse = [&](const char* why) { return fail(SNB_ERR_INVALID_ARGUMENT, std::string(name) + ": " + why); };
+    if (a == nullptr) return refuse("args is null");
     const uint64_t lim = (1ull << 31) - 1;
-    if (a->cols == 0 || a->cols > lim || a->rows > lim)
-        return fail(SNB_ERR_INVALID_ARGUMENT, n + ": rows or cols out of range");
-    if (a->params_len != a->cols) return fail(SNB_ERR_INVALID_ARGUMENT, n + ": params length");
-    if (a->stats_len < a->rows) return fail(SNB_ERR_INVALID_ARGUMENT, n + ": mean and inv_std too small");
-    if (a->gain == nullptr || (a->rows > 0 && (a->mean == nullptr || a->inv_std == nullptr)))
-        return fail(SNB_ERR_INVALID_ARGUMENT, n + ": null pointer");
+    if (a->cols == 0 || a->cols > lim || a->rows > lim) return refuse("rows or cols out of range");
+    if (a->params_len != a->cols) return refuse("params length");
+    if (a->stats_len < a->rows) return refuse("mean and inv_std too small");
+    if (a->gain == nullptr || (a->rows > 0 && (a->mean == nullptr || a->inv_std == nullptr))) return refuse("null pointer");
     for (const void* p : {static_cast<const void*>(a->gain), static_cast<const void*>(a->bias),
                           static_cast<const void*>(a->mean), static_cast<const void*>(a->inv_std),
                           static_cast<const void*>(a->gain_grad), static_cast<const void*>(a->bias_grad)})
-        if (reinterpret_cast<uintptr_t>(p) % 4 != 0)
-            return fail(SNB_ERR_INVALID_ARGUMENT, n + ": a pointer is not aligned to its element");
+        if (reinterpret_cast<uintptr_t>(p) % 4 != 0) return refuse("a pointer is not aligned to its element");
     return check_norm_tensor(name, "input", *a, a->input, a->input_len, a->input_stride, a->input_type,
                              SNB_ERR_INVALID_ARGUMENT);
 }
@@ -847,19 +844,22 @@ int snb_adamw8_step(void* stream, const snb_adamw8_tensor* tensors, uint64_t ten
     if (tensor_count > (1ull << 20)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: too many tensors");
     for (uint64_t i = 0; i < tensor_count; ++i) {
         const snb_adamw8_tensor& t = tensors[i];
-        const std::string at = " in tensor " + std::to_string(i);
+        // (Messages are put together on failure only.)
+        auto refuse = [&](const char* why) {
+            return fail(SNB_ERR_INVALID_ARGUMENT, std::string("adamw8_step: ") + why + " in tensor " + std::to_string(i));
+        };
         if (t.gradient_type != SNB_TYPE_F32 && t.gradient_type != SNB_TYPE_BF16)
-            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: unknown gradient type" + at);
-        if (t.count > (1ull << 40)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: too many elements" + at);
+            return refuse("unknown gradient type");
+        if (t.count > (1ull << 40)) return refuse("too many elements");
         if (t.count > 0 && (t.parameter == nullptr || t.gradient == nullptr || t.first == nullptr ||
                             t.first_scale == nullptr || t.second == nullptr || t.second_scale == nullptr))
-            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: null pointer" + at);
+            return refuse("null pointer");
         const uint64_t words = reinterpret_cast<uintptr_t>(t.parameter) | reinterpret_cast<uintptr_t>(t.first_scale) |
                                reinterpret_cast<uintptr_t>(t.second_scale) |
                                (t.gradient_type == SNB_TYPE_F32 ? reinterpret_cast<uintptr_t>(t.gradient) : 0);
         const uint64_t halves = reinterpret_cast<uintptr_t>(t.gradient) | reinterpret_cast<uintptr_t>(t.shadow);
         if (words % 4 != 0 || halves % 2 != 0)
-            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: a pointer is not aligned to its element" + at);
+            return refuse("a pointer is not aligned to its element");
     }
     if (!(max_gradient_norm > 0.0f)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: max_gradient_norm <= 0");
     if (hyper->step == 0) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_step: steps count from 1");
@@ -880,14 +880,16 @@ int snb_adamw8_moments(void* stream, const snb_adamw8_moments_out* tensors, uint
     if (tensor_count > 0 && tensors == nullptr) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: null pointer");
     for (uint64_t i = 0; i < tensor_count; ++i) {
         const snb_adamw8_moments_out& t = tensors[i];
-        const std::string at = " in tensor " + std::to_string(i);
-        if (t.count > (1ull << 40)) return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: too many elements" + at);
+        auto refuse = [&](const char* why) {
+            return fail(SNB_ERR_INVALID_ARGUMENT, std::string("adamw8_moments: ") + why + " in tensor " + std::to_string(i));
+        };
+        if (t.count > (1ull << 40)) return refuse("too many elements");
         if (t.count > 0 && (t.first == nullptr || t.first_scale == nullptr || t.second == nullptr ||
                             t.second_scale == nullptr || t.first_out == nullptr || t.second_out == nullptr))
-            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: null pointer" + at);
+            return refuse("null pointer");
         if ((reinterpret_cast<uintptr_t>(t.first_scale) | reinterpret_cast<uintptr_t>(t.second_scale) |
              reinterpret_cast<uintptr_t>(t.first_out) | reinterpret_cast<uintptr_t>(t.second_out)) % 4 != 0)
-            return fail(SNB_ERR_INVALID_ARGUMENT, "adamw8_moments: a pointer is not aligned to its element" + at);
+            return refuse("a pointer is not aligned to its element");
     }
     std::string err;
     const int rc = adamw8_moments_launch(static_cast<cudaStream_t>(stream), tensors, tensor_count, &err);

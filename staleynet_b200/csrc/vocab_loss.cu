@@ -498,8 +498,8 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.few_blocks = a.weight_transposed ? std::min<uint64_t>((a.classes + 31) / 32, 4ull * sms)
                                        : (a.classes + 32 * per16 - 1) / (32 * per16);
     l.k_logits = l.f32 ? 3 * l.seg : a.width;
-    // The weight's gradient multiplies by the hidden rows without a target too: those have to be zero then.
-    l.pack_hidden = !l.few && (l.f32 || a.weight_grad != nullptr || !aligned16(a.hidden) || a.hidden_stride % per16 != 0);
+    // Gradients need the hidden rows without a target to be zero: both their logits and the weight's gradient read them.
+    l.pack_hidden = !l.few && (l.f32 || l.gradients || !aligned16(a.hidden) || a.hidden_stride % per16 != 0);
     // (The hidden gradient's product has `seg` columns: those past the width must be zeros of a packed weight.)
     l.pack_weight = !l.few && (l.f32 || !aligned16(a.weight) || a.weight_stride % per16 != 0 ||
                                (a.hidden_grad != nullptr && a.width != l.seg));

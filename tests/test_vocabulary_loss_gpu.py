@@ -135,6 +135,9 @@ def test_rows_without_a_target_may_hold_anything(dtype):
     hidden[targets < 0] = float("nan")
     hidden[(targets < 0).nonzero()[0]] = float("inf")
     _check(hidden, weight, targets, Storage.TRANSPOSED)
+    alone = torch.empty_like(hidden)
+    _run(hidden, weight, targets, Storage.TRANSPOSED, d_hidden=alone)
+    assert bool(alone.isfinite().all()) and not alone[targets < 0].any()
     targets.fill_(-1)
     dh, dw = torch.ones_like(hidden), torch.ones_like(weight)
     losses, total = _run(hidden, weight, targets, Storage.TRANSPOSED, d_hidden=dh, d_weight=dw)
@@ -205,8 +208,10 @@ def test_one_gradient_alone_equals_the_same_gradient_of_both():
     assert torch.equal(both_h, one_h) and torch.equal(both_w, one_w)
 
 
-def test_deterministic_gradients_are_bit_identical():
-    hidden, weight, targets = _case(2048, 192, 3000, BF16, Storage.TRANSPOSED)
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+def test_deterministic_gradients_are_bit_identical(dtype):
+    hidden, weight, targets = _case(2048, 192, 3000, dtype, Storage.TRANSPOSED)
+    *_, dh_e, dw_e = _reference(hidden, weight, targets, Storage.TRANSPOSED, 1.0)
     runs = []
     for _ in range(3):
         dh, dw = torch.empty(hidden.shape, device="cuda"), torch.empty(weight.shape, device="cuda")
@@ -214,6 +219,8 @@ def test_deterministic_gradients_are_bit_identical():
         runs.append((dh, dw, losses, total))
     for other in runs[1:]:
         assert all(torch.equal(a, b) for a, b in zip(runs[0], other))
+    _close(runs[0][0], dh_e, GRAD_TOLERANCE[dtype])
+    _close(runs[0][1], dw_e, GRAD_TOLERANCE[dtype])
 
 
 def test_gradients_against_differences():
