@@ -424,9 +424,10 @@ typedef struct snb_vocabulary_loss_args {
 } snb_vocabulary_loss_args;
 
 /* *bytes = the workspace that a call with these arguments needs (the workspace fields are not read): statistics of
- * rows * classes / 16 bytes; for gradients a piece of p of at most 256 MB (or 256 classes), a packed copy of hidden and
- * f32 sums of hidden's size; and where the weight is f32 or not laid out for TMA (16-byte aligned rows), a packed piece
- * of it of at most 256 MB. */
+ * rows * classes / 16 bytes; for gradients a piece of p of at most 768 MB (or 256 classes), a packed copy of hidden and,
+ * unless the hidden gradient is f32 with 16-byte aligned rows, f32 sums of its size; f32 sums of a piece of the weight's
+ * gradient; and where the weight is f32 or not laid out for TMA (16-byte aligned rows), a packed piece of it of at most
+ * 256 MB. It depends on the operands' alignment: ask with the pointers of the call. */
 SNB_API int snb_vocabulary_cross_entropy_workspace(const snb_vocabulary_loss_args* args, uint64_t* bytes);
 
 /* Needs sm_100 tensor cores (SNB_ERR_UNSUPPORTED otherwise). Checks, in this order: sizes and types, lengths, null

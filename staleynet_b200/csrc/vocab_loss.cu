@@ -17,7 +17,8 @@
 // x y = lo hi' + hi lo' + hi hi' up to 2^-22 of |x y|: three TF32 products with f32 sums. The logits take them as one
 // product over three times the width (H packed as lo|hi|hi, W as hi|lo|hi), so that the epilogue sees whole logits; the
 // tensor core cuts off what a sum's last bit cannot hold at every instruction, so the small products come first, where
-// that costs little. The gradient products add one after the other into f32 outputs.
+// that costs little. A gradient product takes its three in one launch, each unit of work the small ones and then at most
+// kSumLength of the large one, added into f32 outputs; or, in the deterministic order, one after the other.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -64,13 +65,20 @@ struct PackParams {
 __device__ __forceinline__ void wait_for_previous_kernel() { asm volatile("griddepcontrol.wait;" ::: "memory"); }
 __device__ __forceinline__ void allow_next_kernel() { asm volatile("griddepcontrol.launch_dependents;" ::: "memory"); }
 
-// The three elementwise kernels take 4 columns (16 bytes of f32) a thread: blockDim.x threads along a row, blockDim.y rows
-// a block, rows in steps of the grid. `vec`: the side that is not in the workspace allows 4-element accesses.
 __device__ __forceinline__ bool has_target(const uint32_t* targets, int64_t row) {
     return targets == nullptr || __ldg(targets + row) != kEmptyToken;
 }
 
+// The three elementwise kernels (the two that pack, and store_kernel) take 4 columns (16 bytes of f32) a thread: blockDim.x
+// threads along a row, blockDim.y rows a block, rows in steps of the grid. `vec`: the side that is not in the workspace
+// allows 4-element accesses. Memory bounds them; at the sizes where they are needed, a launch's few microseconds do: packing
+// 8,192 x 768 bf16 takes 9 us (25 MB, 2.8 TB/s), splitting 10,007 x 256 f32 9 us (41 MB, 4.6 TB/s), storing 8,192 x 768
+// f32 sums as bf16 10.6 us (38 MB, 3.6 TB/s).
+//
+// The pack kernels wait for the kernel before them only at their end: a packed weight may be written while the hidden rows
+// are still being packed, and whoever waits for the weight then waits for both.
 __global__ void __launch_bounds__(256) pack_bf16_kernel(const PackParams p, int vec) {
+    allow_next_kernel();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; i < p.dst_rows;
          i += static_cast<int64_t>(gridDim.x) * blockDim.y) {
         const bool live = i < p.rows && has_target(p.targets, i);
@@ -89,6 +97,7 @@ __global__ void __launch_bounds__(256) pack_bf16_kernel(const PackParams p, int 
             *reinterpret_cast<uint2*>(dst + j) = q;
         }
     }
+    wait_for_previous_kernel();
 }
 
 // The nearest value of 11 significant bits; a finite value that would round past the largest float is cut off instead.
@@ -99,6 +108,7 @@ __device__ __forceinline__ float tf32_nearest(float x) {
 }
 
 __global__ void __launch_bounds__(256) pack_split_kernel(const PackParams p, int vec) {
+    allow_next_kernel();
     for (int64_t i = static_cast<int64_t>(blockIdx.x) * blockDim.y + threadIdx.y; i < p.dst_rows;
          i += static_cast<int64_t>(gridDim.x) * blockDim.y) {
         const bool live = i < p.rows && has_target(p.targets, i);
@@ -126,6 +136,7 @@ __global__ void __launch_bounds__(256) pack_split_kernel(const PackParams p, int
                     (p.low >> k) & 1 ? make_float4(lo[0], lo[1], lo[2], lo[3]) : make_float4(hi[0], hi[1], hi[2], hi[3]);
         }
     }
+    wait_for_previous_kernel();
 }
 
 // out[i, j] (+)= ws[i, j] for i < rows, j < cols; the workspace's rows are multiples of 4 elements.
@@ -173,7 +184,10 @@ __device__ __forceinline__ void join(float2& a, float2 b) {
 // 32 warps take every 32nd pair; then a warp for each row joins the 32 results in a fixed tree, so the result does not
 // depend on scheduling. Writes the row's loss and, for pass 2, (log2 e maximum, log2 sum), with a maximum of +inf in a row
 // without a target (every exponential is then 0) and NaN for a target that is no class. A grid of one block also writes
-// the sum of the losses.
+// the sum of the losses. (Having the block that finishes last write it for larger grids, by a ticket, measured no faster
+// than loss_sum_kernel, whose launch hides behind this kernel: 189.8 against 189.1 us for 4,096 x 512 x 50,021 bf16.)
+//   Bound by the latency of the chain read, join, tree: 6.5 us for one row of 32,000 classes, 9 us for 8,192 rows of
+// 32,768 (17 MB).
 __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     combine_kernel(const float2* partials, int64_t pairs, int64_t rows, const uint32_t* targets, uint64_t classes,
                    const float* target_logit, float* losses, float2* row_stats, float* loss_sum) {
@@ -470,6 +484,7 @@ struct Layout {
     uint64_t hidden_ld, weight_ld;   // of the operands that the products read
     uint64_t grad_ld;       // of a piece of P
     uint64_t wgrad_ld, wgrad_rows;   // f32 weight gradient of a piece before it is stored
+    bool hidden_grad_direct;         // dH is summed where the caller wants it
     uint64_t hidden_at, weight_at, partials_at, target_at, stats_at, p_at, dh_at, dw_at, bytes;
 };
 
@@ -535,6 +550,7 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.grad_ld = piece_ld;
     l.wgrad_rows = a.weight_transposed ? l.piece : l.seg;
     l.wgrad_ld = a.weight_transposed ? l.seg : piece_ld;
+    l.hidden_grad_direct = a.hidden_grad_type == SNB_TYPE_F32 && aligned16(a.hidden_grad) && a.width % 4 == 0;
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -548,7 +564,7 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.target_at = take(a.rows * 4);
     l.stats_at = take(a.rows * sizeof(float2));
     l.p_at = take(l.gradients ? a.rows * l.grad_ld * (l.f32 ? 8 : 2) : 0);
-    l.dh_at = take(a.hidden_grad != nullptr ? a.rows * l.seg * 4 : 0);
+    l.dh_at = take(a.hidden_grad != nullptr && !l.hidden_grad_direct ? a.rows * l.seg * 4 : 0);
     l.dw_at = take(a.weight_grad != nullptr ? l.wgrad_rows * l.wgrad_ld * 4 : 0);
     l.bytes = a.rows == 0 ? 0 : at + 256;
     return l;
@@ -606,7 +622,7 @@ struct Call {
     };
 
     int pack(const void* src, uint64_t src_ld, uint64_t rows, uint64_t cols, void* dst, uint64_t dst_ld,
-             uint64_t dst_rows, uint64_t dst_cols, const uint32_t* targets, uint64_t plane, int low) const {
+             uint64_t dst_rows, uint64_t dst_cols, const uint32_t* targets, uint64_t plane, int low, bool early) const {
         PackParams p{};
         p.src = src;
         p.src_ld = static_cast<int64_t>(src_ld);
@@ -622,8 +638,9 @@ struct Call {
         const dim3 threads = row_threads(dst_cols);
         const unsigned grid = row_blocks(dst_rows, threads, sms);
         const int vec = reinterpret_cast<uintptr_t>(src) % (4 * l.elem) == 0 && src_ld % 4 == 0;
-        if (l.f32) pack_split_kernel<<<grid, threads, 0, stream>>>(p, vec);
-        else pack_bf16_kernel<<<grid, threads, 0, stream>>>(p, vec);
+        const auto kernel = l.f32 ? pack_split_kernel : pack_bf16_kernel;
+        if (early) launch_early(kernel, grid, threads, stream, p, vec);
+        else kernel<<<grid, threads, 0, stream>>>(p, vec);
         return launched("vocabulary loss pack kernel launch", err);
     }
 
@@ -644,8 +661,9 @@ struct Call {
         return l.f32 ? Part{p, static_cast<const float*>(p) + a.rows * l.grad_ld} : Part{p, nullptr};
     }
 
-    // The weight of the classes from v0 on, packed into the workspace where the products cannot read it in place.
-    int weight(uint64_t v0, uint64_t n, const void** w) const {
+    // The weight of the classes from v0 on, packed into the workspace where the products cannot read it in place. early:
+    // the kernel before it on the stream packs the hidden rows.
+    int weight(uint64_t v0, uint64_t n, const void** w, bool early = false) const {
         const uint64_t offset = (a.weight_transposed ? v0 * a.weight_stride : v0) * l.elem;
         const void* src = static_cast<const uint8_t*>(a.weight) + offset;
         *w = src;
@@ -653,9 +671,10 @@ struct Call {
         *w = at(l.weight_at);
         constexpr int kHiLoHi = 2;
         if (a.weight_transposed)
-            return pack(src, a.weight_stride, n, a.width, at(l.weight_at), l.weight_ld, n, l.seg, nullptr, l.seg, kHiLoHi);
+            return pack(src, a.weight_stride, n, a.width, at(l.weight_at), l.weight_ld, n, l.seg, nullptr, l.seg, kHiLoHi,
+                        early);
         return pack(src, a.weight_stride, a.width, n, at(l.weight_at), l.weight_ld, l.seg, round_up(n, 8), nullptr,
-                    l.seg * l.weight_ld, kHiLoHi);
+                    l.seg * l.weight_ld, kHiLoHi, early);
     }
 
     VocabProduct logits(uint64_t v0, uint64_t n, const void* w) const {
@@ -757,11 +776,14 @@ struct Call {
         return launched("vocabulary loss store kernel launch", err);
     }
 
-    // dH (+)= P W of one piece, into the f32 sums.
+    // dH (+)= P W of one piece, in f32: in the caller's gradient, or in the workspace with rows of `seg` columns. (The first,
+    // and packing both operands side by side, took a call of 1,021 x 256 x 10,007 f32 from 174 to 169 us.)
     int hidden_grad(uint64_t v0, uint64_t n, const void* w) const {
         const snb_operand left{l.grad_ld, 1, 0};
         const snb_operand right = a.weight_transposed ? snb_operand{l.weight_ld, 1, 0} : snb_operand{1, l.weight_ld, 0};
-        return product(a.rows, l.seg, n, grad_part(), left, weight_part(w), right, at(l.dh_at), SNB_TYPE_F32, v0 > 0);
+        const bool direct = l.hidden_grad_direct;
+        return product(a.rows, direct ? a.width : l.seg, n, grad_part(), left, weight_part(w), right,
+                       direct ? a.hidden_grad : at(l.dh_at), SNB_TYPE_F32, v0 > 0);
     }
 
     // Whether an output's tiles, unsplit, keep three fifths of the CTA pairs' rounds busy.
@@ -850,7 +872,7 @@ struct Call {
         constexpr int kLoHiHi = 1;
         if (l.pack_hidden) {
             rc = pack(a.hidden, a.hidden_stride, a.rows, a.width, at(l.hidden_at), l.hidden_ld, a.rows, l.seg,
-                      l.gradients ? a.targets : nullptr, l.seg, kLoHiHi);
+                      l.gradients ? a.targets : nullptr, l.seg, kLoHiHi, false);
             if (rc != SNB_OK) return rc;
         }
         // Pass 1: a weight that is read in place needs no pieces here.
@@ -859,7 +881,7 @@ struct Call {
         if (l.few && (rc = few()) != SNB_OK) return rc;
         for (uint64_t v0 = 0; v0 < a.classes && !l.few; v0 += step) {
             const uint64_t n = std::min(step, a.classes - v0);
-            if ((rc = weight(v0, n, &w)) != SNB_OK) return rc;
+            if ((rc = weight(v0, n, &w, l.pack_hidden && v0 == 0)) != SNB_OK) return rc;
             if ((rc = tc_vocab_product(stream, logits(v0, n, w), err)) != SNB_OK) return rc;
         }
         const uint64_t blocks = (a.rows + kCombineRows - 1) / kCombineRows;
@@ -885,9 +907,8 @@ struct Call {
             if (a.weight_grad != nullptr && (rc = weight_grad(v0, n)) != SNB_OK) return rc;
             if (a.hidden_grad != nullptr && (rc = hidden_grad(v0, n, w)) != SNB_OK) return rc;
         }
-        return a.hidden_grad == nullptr ? SNB_OK
-                                        : store(at(l.dh_at), l.seg, a.hidden_grad, a.hidden_grad_type, a.width, a.rows,
-                                                a.width, false);
+        if (a.hidden_grad == nullptr || l.hidden_grad_direct) return SNB_OK;
+        return store(at(l.dh_at), l.seg, a.hidden_grad, a.hidden_grad_type, a.width, a.rows, a.width, false);
     }
 };
 
