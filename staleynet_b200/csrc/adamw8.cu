@@ -17,8 +17,9 @@
 // Step. As the reference's (kernels/optimizer.rs:57-70) on g = gradient times the clip factor max_norm / norm; the norm is
 // that of all tensors together, its squares summed in f64 in a fixed order, so steps are the same from run to run.
 //
-// What bounds it: memory. An element's parameter (4 bytes read, 4 written, and 2 for its bf16 copy), gradient (2 or 4,
-// twice: once for the norm) and two codes (2 read, 2 written).
+// What bounds it: memory, an element's parameter (4 bytes read, 4 written, and 2 for its bf16 copy), gradient (2 or 4,
+// twice: once for the norm) and two codes (2 read, 2 written); and in the step nearly as much the issue of its
+// instructions, about a hundred for an element, most of them for the two roundings.
 #include <cuda_runtime.h>
 
 #include <algorithm>
@@ -33,27 +34,53 @@ namespace {
 
 constexpr int kBlock = 256;             // elements that share a scale
 constexpr int kWarps = 8;               // warps of a thread block
-constexpr int kChunk = 4 * kWarps * kBlock;  // elements that a thread block takes at a time
+constexpr int kPart = kWarps * kBlock;  // elements that a thread block takes at once
 constexpr int kStepBlocks = 3;          // thread blocks of the step that are resident on an SM (80 registers a thread)
 constexpr int kMaxTensors = 256;        // of one launch (its table is a kernel parameter)
-constexpr int kSumBlocks = 592;         // thread blocks of the norm's sum, and partial sums of one launch
+constexpr int kSumBlocks = 888;         // thread blocks of the norm's sum, and partial sums of one launch: six an SM (97.6
+                                        // million f32 gradients: 77 us; 80 us on three an SM, 78 on eight)
 constexpr uint64_t kGolden = 0x9E3779B97F4A7C15ull;
+
+// How a launch's grid shares the parts of its tensors: a contiguous run each, `longer` blocks one part more than the rest.
+// The tensor in which each run begins comes from the host, since a search through the table in every block would wait for
+// one uncached constant after the other. (Blocks that took every gridDim.x-th piece of 8,192 elements, with that search at
+// each, were slower: 434 us for a step on 97.6 million elements that takes 418 us here.)
+constexpr int kMaxGrid = 2048;
+struct Shares {
+    int64_t each, longer;
+    uint8_t first_tensor[kMaxGrid];
+};
 
 struct Table {
     int32_t n;
+    Shares shares;
     snb_adamw8_tensor t[kMaxTensors];
-    int64_t chunk_start[kMaxTensors + 1];
+    int64_t part_start[kMaxTensors + 1];
 };
 static_assert(sizeof(Table) < 32000, "kernel parameters");
 
-__device__ __forceinline__ int tensor_of_chunk(const int64_t* chunk_start, int n, int64_t chunk) {
-    int lo = 0, hi = n - 1;
-    while (lo < hi) {  // last tensor that starts at or before the chunk (an empty one starts where the next does)
-        const int mid = (lo + hi + 1) >> 1;
-        if (chunk_start[mid] <= chunk) lo = mid;
-        else hi = mid - 1;
-    }
-    return lo;
+// A thread block's share, through which it walks tensor by tensor.
+struct Share {
+    int64_t part, end;  // the run's next part and its end
+    int tensor;         // that holds `part`
+};
+
+template <typename T>
+__device__ __forceinline__ Share share_of(const T& m) {
+    const int64_t b = blockIdx.x, part = b * m.shares.each + min(b, m.shares.longer);
+    return {part, part + m.shares.each + (b < m.shares.longer ? 1 : 0), m.shares.first_tensor[b]};
+}
+
+// The end of the run within its current tensor, in elements.
+template <typename T>
+__device__ __forceinline__ int64_t end_of(const T& m, const Share& s) {
+    return min((s.end - m.part_start[s.tensor]) * kPart, static_cast<int64_t>(m.t[s.tensor].count));
+}
+
+template <typename T>
+__device__ __forceinline__ void next_tensor(const T& m, Share& s) {
+    s.part = m.part_start[++s.tensor];
+    while (s.part < s.end && m.part_start[s.tensor + 1] == s.part) ++s.tensor;
 }
 
 __device__ __forceinline__ float bf16_value(uint16_t h) { return __uint_as_float(static_cast<uint32_t>(h) << 16); }
@@ -182,14 +209,14 @@ __device__ __forceinline__ double block_sum(double v) {
     return sum;
 }
 
+// The sum of the squares of all gradients, a partial sum for each thread block. Bound by memory: 97.6 million f32 gradients
+// (391 MB, 60 us at the copy rate) take 77 us; 4.8 million bf16 ones, a latency, 6.3 us.
 __global__ void __launch_bounds__(32 * kWarps) adamw8_norm_kernel(const __grid_constant__ Table m, double* partials) {
-    const int64_t chunks = m.chunk_start[m.n];
     double sum = 0.0;
-    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-        const int t = tensor_of_chunk(m.chunk_start, m.n, chunk);
-        const snb_adamw8_tensor& x = m.t[t];
-        const int64_t begin = (chunk - m.chunk_start[t]) * kChunk;
-        const int64_t n = min(static_cast<int64_t>(x.count) - begin, static_cast<int64_t>(kChunk));
+    for (Share s = share_of(m); s.part < s.end; next_tensor(m, s)) {
+        const snb_adamw8_tensor& x = m.t[s.tensor];
+        const int64_t begin = (s.part - m.part_start[s.tensor]) * kPart;
+        const int64_t n = end_of(m, s) - begin;
         const bool bf16 = x.gradient_type == SNB_TYPE_BF16;
         int64_t scalar_begin = 0;
         if (bf16 && multiple(x.gradient, 16)) {
@@ -205,7 +232,7 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_norm_kernel(const __grid_c
             scalar_begin = n / 8 * 8;
         } else if (!bf16 && multiple(x.gradient, 16)) {
             const float4* g = reinterpret_cast<const float4*>(static_cast<const float*>(x.gradient) + begin);
-#pragma unroll 4
+#pragma unroll 8
             for (int64_t i = threadIdx.x; i < n / 4; i += 32 * kWarps) {
                 const float4 q = __ldg(g + i);
                 for (double v : {static_cast<double>(q.x), static_cast<double>(q.y), static_cast<double>(q.z),
@@ -235,6 +262,11 @@ struct StepParams {
     double* square_sum;
 };
 
+// The step. A warp takes the 256 elements that share a scale, eight a lane, and holds them in registers from the read to the
+// code, since the new scale is known only when the last of them is. 97.6 million elements with f32 gradients and bf16 copies
+// (1.76 GB, 272 us at the copy rate) take 418 us, with the arithmetic and the memory traffic (348 us alone) overlapping for
+// the most part; three resident blocks an SM at 80 registers, against 469 us for two. 4.8 million elements with bf16
+// gradients (76 MB): 28 us, bound by the latency of five passes of a warp.
 __global__ void __launch_bounds__(32 * kWarps, kStepBlocks) adamw8_step_kernel(const __grid_constant__ Table m, const StepParams a) {
     // Every thread block adds the norm's partial sums in the same order.
     double sum = 0.0;
@@ -245,16 +277,14 @@ __global__ void __launch_bounds__(32 * kWarps, kStepBlocks) adamw8_step_kernel(c
     const float clip = norm > a.max_norm ? __fdiv_rn(a.max_norm, norm) : 1.0f;
 
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t chunks = m.chunk_start[m.n];
-    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-        const int t = tensor_of_chunk(m.chunk_start, m.n, chunk);
-        const snb_adamw8_tensor& x = m.t[t];
-        const int64_t begin = (chunk - m.chunk_start[t]) * kChunk;
+    for (Share s = share_of(m); s.part < s.end; next_tensor(m, s)) {
+        const snb_adamw8_tensor& x = m.t[s.tensor];
+        const int64_t begin = (s.part - m.part_start[s.tensor]) * kPart, end = end_of(m, s);
         const int64_t count = static_cast<int64_t>(x.count);
         const bool grad_bf16 = x.gradient_type == SNB_TYPE_BF16;
         const bool aligned = multiple(x.parameter, 16) && multiple(x.gradient, grad_bf16 ? 8 : 16) &&
                              multiple(x.first, 4) && multiple(x.second, 4) && multiple(x.shadow, 8);
-        for (int64_t at = begin + warp * kBlock; at < min(begin + kChunk, count); at += kWarps * kBlock) {
+        for (int64_t at = begin + warp * kBlock; at < end; at += kPart) {
             const bool whole = aligned && at + kBlock <= count;
             float w[8], g[8];
             uint32_t c1[2] = {0, 0}, c2[2] = {0, 0};
@@ -394,25 +424,29 @@ __global__ void __launch_bounds__(32 * kWarps, kStepBlocks) adamw8_step_kernel(c
     }
 }
 
-// The moments' values in f32, for checkpoints and inspection.
+// The moments' values in f32, for checkpoints and inspection. Bound by memory, most of it the 8 bytes written for an element:
+// 97.6 million elements (976 MB, 151 us at the copy rate) take 164 us on three blocks an SM; four, whose writes go to more
+// places at once, take 174 us and eight 178 us. Where L2 holds the values more blocks do no harm and hide more latency:
+// 4.8 million elements take 10.4 us on eight, 12.1 us on three.
+constexpr int64_t kCachedBytes = 96 << 20;
+
 struct MomentTable {
     int32_t n;
+    Shares shares;
     snb_adamw8_moments_out t[kMaxTensors];
-    int64_t chunk_start[kMaxTensors + 1];
+    int64_t part_start[kMaxTensors + 1];
 };
 static_assert(sizeof(MomentTable) < 32000, "kernel parameters");
 
 __global__ void __launch_bounds__(32 * kWarps) adamw8_moments_kernel(const __grid_constant__ MomentTable m) {
     const int lane = threadIdx.x & 31, warp = threadIdx.x >> 5;
-    const int64_t chunks = m.chunk_start[m.n];
-    for (int64_t chunk = blockIdx.x; chunk < chunks; chunk += gridDim.x) {
-        const int t = tensor_of_chunk(m.chunk_start, m.n, chunk);
-        const snb_adamw8_moments_out& x = m.t[t];
-        const int64_t begin = (chunk - m.chunk_start[t]) * kChunk;
+    for (Share s = share_of(m); s.part < s.end; next_tensor(m, s)) {
+        const snb_adamw8_moments_out& x = m.t[s.tensor];
+        const int64_t begin = (s.part - m.part_start[s.tensor]) * kPart, end = end_of(m, s);
         const int64_t count = static_cast<int64_t>(x.count);
         const bool aligned = multiple(x.first, 4) && multiple(x.second, 4) && multiple(x.first_out, 16) &&
                              multiple(x.second_out, 16);
-        for (int64_t at = begin + warp * kBlock; at < min(begin + kChunk, count); at += kWarps * kBlock) {
+        for (int64_t at = begin + warp * kBlock; at < end; at += kPart) {
             const float s1 = x.first_scale[at / kBlock], s2 = x.second_scale[at / kBlock];
             auto value1 = [&](int8_t c) {
                 const float q = static_cast<float>(c);
@@ -423,17 +457,22 @@ __global__ void __launch_bounds__(32 * kWarps) adamw8_moments_kernel(const __gri
                 return __fmul_rn(__fmul_rn(root, root), s2);
             };
             if (aligned && at + kBlock <= count) {
+                uint32_t c1[2], c2[2];
 #pragma unroll
                 for (int h = 0; h < 2; ++h) {
                     const int64_t e = at + element_of(lane, 4 * h);
-                    const uint32_t c1 = *reinterpret_cast<const uint32_t*>(x.first + e);
-                    const uint32_t c2 = *reinterpret_cast<const uint32_t*>(x.second + e);
+                    c1[h] = *reinterpret_cast<const uint32_t*>(x.first + e);
+                    c2[h] = *reinterpret_cast<const uint32_t*>(x.second + e);
+                }
+#pragma unroll
+                for (int h = 0; h < 2; ++h) {
+                    const int64_t e = at + element_of(lane, 4 * h);
                     *reinterpret_cast<float4*>(x.first_out + e) =
-                        make_float4(value1(static_cast<int8_t>(c1)), value1(static_cast<int8_t>(c1 >> 8)),
-                                    value1(static_cast<int8_t>(c1 >> 16)), value1(static_cast<int8_t>(c1 >> 24)));
+                        make_float4(value1(static_cast<int8_t>(c1[h])), value1(static_cast<int8_t>(c1[h] >> 8)),
+                                    value1(static_cast<int8_t>(c1[h] >> 16)), value1(static_cast<int8_t>(c1[h] >> 24)));
                     *reinterpret_cast<float4*>(x.second_out + e) =
-                        make_float4(value2(c2 & 0xFFu), value2((c2 >> 8) & 0xFFu), value2((c2 >> 16) & 0xFFu),
-                                    value2(c2 >> 24));
+                        make_float4(value2(c2[h] & 0xFFu), value2((c2[h] >> 8) & 0xFFu), value2((c2[h] >> 16) & 0xFFu),
+                                    value2(c2[h] >> 24));
                 }
             } else {
                 for (int j = 0; j < 8; ++j) {
@@ -458,15 +497,31 @@ int launched(const char* what, std::string* err) {
 template <typename T, typename Source>
 uint64_t fill(T* table, const Source* tensors, uint64_t first, uint64_t n) {
     const uint64_t take = std::min<uint64_t>(n - first, kMaxTensors);
-    int64_t chunks = 0;
+    int64_t parts = 0;
     for (uint64_t i = 0; i < take; ++i) {
         table->t[i] = tensors[first + i];
-        table->chunk_start[i] = chunks;
-        chunks += static_cast<int64_t>((tensors[first + i].count + kChunk - 1) / kChunk);
+        table->part_start[i] = parts;
+        parts += static_cast<int64_t>((tensors[first + i].count + kPart - 1) / kPart);
     }
-    table->chunk_start[take] = chunks;
+    table->part_start[take] = parts;
     table->n = static_cast<int32_t>(take);
     return take;
+}
+
+// Shares a table's parts between at most `most` blocks; returns how many.
+template <typename T>
+unsigned share(T* table, int64_t most) {
+    const int64_t parts = table->part_start[table->n];
+    const int64_t blocks = std::min<int64_t>(parts, std::min<int64_t>(most, kMaxGrid));
+    table->shares.each = parts / blocks;
+    table->shares.longer = parts % blocks;
+    int tensor = 0;
+    for (int64_t b = 0, part = 0; b < blocks; ++b) {
+        while (table->part_start[tensor + 1] <= part) ++tensor;
+        table->shares.first_tensor[b] = static_cast<uint8_t>(tensor);
+        part += table->shares.each + (b < table->shares.longer ? 1 : 0);
+    }
+    return static_cast<unsigned>(blocks);
 }
 
 }  // namespace
@@ -485,9 +540,8 @@ int adamw8_step_launch(cudaStream_t s, const snb_adamw8_tensor* tensors, uint64_
     int32_t sums = 0;
     for (uint64_t i = 0; i < n; i += kMaxTensors) {
         fill(&table, tensors, i, n);
-        const int64_t chunks = table.chunk_start[table.n];
-        if (chunks == 0) continue;
-        const int blocks = static_cast<int>(std::min<int64_t>(chunks, kSumBlocks));
+        if (table.part_start[table.n] == 0) continue;
+        const unsigned blocks = share(&table, kSumBlocks);
         adamw8_norm_kernel<<<blocks, 32 * kWarps, 0, s>>>(table, partials + sums);
         if ((rc = launched("adamw8_norm_kernel launch", err)) != SNB_OK) return rc;
         sums += blocks;
@@ -525,10 +579,9 @@ int adamw8_step_launch(cudaStream_t s, const snb_adamw8_tensor* tensors, uint64_
     a.square_sum = square_sum;
     for (uint64_t i = 0; i < n; i += kMaxTensors) {
         if (n > kMaxTensors) fill(&table, tensors, i, n);
-        const int64_t chunks = table.chunk_start[table.n];
-        if (chunks == 0) continue;
-        const int64_t blocks = std::min<int64_t>(chunks, static_cast<int64_t>(kStepBlocks) * dev.sm_count);
-        adamw8_step_kernel<<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(table, a);
+        if (table.part_start[table.n] == 0) continue;
+        const unsigned blocks = share(&table, kStepBlocks * dev.sm_count);
+        adamw8_step_kernel<<<blocks, 32 * kWarps, 0, s>>>(table, a);
         if ((rc = launched("adamw8_step_kernel launch", err)) != SNB_OK) return rc;
     }
     return SNB_OK;
@@ -541,10 +594,10 @@ int adamw8_moments_launch(cudaStream_t s, const snb_adamw8_moments_out* tensors,
     MomentTable table{};
     for (uint64_t i = 0; i < n; i += kMaxTensors) {
         fill(&table, tensors, i, n);
-        const int64_t chunks = table.chunk_start[table.n];
-        if (chunks == 0) continue;
-        const int64_t blocks = std::min<int64_t>(chunks, 8ll * dev.sm_count);
-        adamw8_moments_kernel<<<static_cast<unsigned>(blocks), 32 * kWarps, 0, s>>>(table);
+        if (table.part_start[table.n] == 0) continue;
+        const bool cached = table.part_start[table.n] * kPart * 8 <= kCachedBytes;
+        const unsigned blocks = share(&table, (cached ? 8 : 3) * dev.sm_count);
+        adamw8_moments_kernel<<<blocks, 32 * kWarps, 0, s>>>(table);
         if ((rc = launched("adamw8_moments_kernel launch", err)) != SNB_OK) return rc;
     }
     return SNB_OK;

@@ -282,6 +282,11 @@ struct NormParams {
 
 // Both kernels: T threads a row, NE elements a thread, `depth` rows in flight in shared memory (a ring for each warp when
 // T is 32, else one of the block), rows first, first + step, ... . kMaxDepth bounds the waits' immediate operands.
+//
+// Measured. Forward, 65,536 x 768 bf16 (202 MB, 31 us at the copy rate): 33 us; one row of 768 f32: 2.4 us, a launch.
+// Backward, 65,536 x 768 bf16 (302 MB, 47 us at the copy rate): 51 us; 4,096 x 256 f32: 4.1 us; 3,001 x 5,003 bf16, whose
+// rows start off every boundary (90 MB, 14 us): 29 us, bound by the chain of each row, which two barriers interrupt, and by
+// its single-element reads from shared memory.
 constexpr int kMaxDepth = 4;
 
 __device__ __forceinline__ void wait_for_row(int depth) {
@@ -536,7 +541,8 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T <= 256 ? 
 }
 
 // out[c] (+)= the sum of sums[0 .. parts, c], in a fixed order: a block's 32 warps take every 32nd part of 32 columns.
-// blockIdx.y: 0 the gain's gradient, 1 the bias's.
+// blockIdx.y: 0 the gain's gradient, 1 the bias's. Bound by the latency of its few reads: 5 to 6 us for 768 columns of 296
+// parts, 8.5 us for 5,003 (12 MB). Ten reads at a time or half the warps moved the whole pass by less than 2 % either way.
 __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* sums, int64_t parts, int64_t cols,
                                                                   float* gain_grad, float* bias_grad, int accumulate) {
     __shared__ float part[32][33];
@@ -559,7 +565,8 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* s
     out[c] = accumulate ? out[c] + s : s;
 }
 
-// Rows of any length, a block each, read three times (forward) or twice (backward).
+// Rows of any length, a block each, read three times (forward) or twice (backward). What binds them is those passes, which
+// mostly hit L1 and L2; they stand for rows that the shapes below have no registers for.
 constexpr int kWideThreads = 512;
 
 __device__ __forceinline__ float element(const void* row, int64_t c, bool bf16) {
