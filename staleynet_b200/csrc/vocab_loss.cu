@@ -200,8 +200,23 @@ __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     float2 v = make_float2(-inf, 0.0f);
     const int64_t read_row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
     if (read_row < rows) {
-#pragma unroll 4
-        for (int64_t k = w; k < pairs; k += kCombineLanes) join(v, partials[k * rows + read_row]);
+        // Several pairs at a time: their reads overlap, and all but one factor of their sums are independent of each other.
+        constexpr int kBatch = 8;
+        for (int64_t k = w; k < pairs; k += kBatch * kCombineLanes) {
+            float2 in[kBatch];
+            float next = v.x;
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) {
+                const int64_t pair = k + i * kCombineLanes;
+                in[i] = pair < pairs ? partials[pair * rows + read_row] : make_float2(-inf, 0.0f);
+                next = fmaxf(next, in[i].x);
+            }
+            const float base = next == -inf ? 0.0f : __fmul_rn(next, kLog2e);
+            v.y *= exp2f(__fmul_rn(v.x, kLog2e) - base);
+#pragma unroll
+            for (int i = 0; i < kBatch; ++i) v.y += in[i].y * exp2f(__fmul_rn(in[i].x, kLog2e) - base);
+            v.x = next;
+        }
     }
     part[w][r] = v;
     __syncthreads();
