@@ -412,7 +412,7 @@ typedef struct snb_vocabulary_loss_args {
     float* loss_sum;           /* their sum, in a fixed order; or NULL */
     float grad_scale;
     int32_t flags;             /* SNB_GEMM_DETERMINISTIC: bit-identical gradients from run to run; or 0 */
-    void* hidden_grad;         /* [rows, width], overwritten; or NULL */
+    void* hidden_grad;         /* [rows, width], overwritten (it may be hidden itself); or NULL */
     uint64_t hidden_grad_len;
     void* weight_grad;         /* dense, in the weight's order; or NULL */
     uint64_t weight_grad_len;

@@ -59,6 +59,8 @@ struct PackParams {
     const uint32_t* targets;
     int64_t plane[3];
     int32_t low;
+    uint4* zero[2];         // f32: arrays that become zeros on the way, of zero_count 16-byte pieces
+    int64_t zero_count[2];
 };
 
 // Small kernels start while the kernel before them drains (programmatic launch) and wait for it here.
@@ -136,6 +138,11 @@ __global__ void __launch_bounds__(256) pack_split_kernel(const PackParams p, int
                     (p.low >> k) & 1 ? make_float4(lo[0], lo[1], lo[2], lo[3]) : make_float4(hi[0], hi[1], hi[2], hi[3]);
         }
     }
+    const int64_t thread = threadIdx.y * blockDim.x + threadIdx.x, block = blockDim.x * blockDim.y;
+#pragma unroll
+    for (int z = 0; z < 2; ++z)
+        for (int64_t i = blockIdx.x * block + thread; i < p.zero_count[z]; i += gridDim.x * block)
+            p.zero[z][i] = make_uint4(0, 0, 0, 0);
     wait_for_previous_kernel();
 }
 
@@ -500,6 +507,7 @@ struct Layout {
     uint64_t grad_ld;       // of a piece of P
     uint64_t wgrad_ld, wgrad_rows;   // f32 weight gradient of a piece before it is stored
     bool hidden_grad_direct;         // dH is summed where the caller wants it
+    bool weight_grad_direct;         // so is dW [classes, width]
     uint64_t hidden_at, weight_at, partials_at, target_at, stats_at, p_at, dh_at, dw_at, bytes;
 };
 
@@ -566,6 +574,8 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.wgrad_rows = a.weight_transposed ? l.piece : l.seg;
     l.wgrad_ld = a.weight_transposed ? l.seg : piece_ld;
     l.hidden_grad_direct = a.hidden_grad_type == SNB_TYPE_F32 && aligned16(a.hidden_grad) && a.width % 4 == 0;
+    l.weight_grad_direct = a.weight_transposed != 0 && a.weight_grad_type == SNB_TYPE_F32 && aligned16(a.weight_grad) &&
+                           a.width % 4 == 0;
     uint64_t at = 0;
     auto take = [&](uint64_t bytes) {
         const uint64_t here = at;
@@ -637,8 +647,17 @@ struct Call {
     };
 
     int pack(const void* src, uint64_t src_ld, uint64_t rows, uint64_t cols, void* dst, uint64_t dst_ld,
-             uint64_t dst_rows, uint64_t dst_cols, const uint32_t* targets, uint64_t plane, int low, bool early) const {
+             uint64_t dst_rows, uint64_t dst_cols, const uint32_t* targets, uint64_t plane, int low, bool early,
+             bool zeros = false) const {
         PackParams p{};
+        if (zeros && zero_hidden_grad()) {
+            p.zero[0] = static_cast<uint4*>(hidden_sums());
+            p.zero_count[0] = static_cast<int64_t>(a.rows * (l.hidden_grad_direct ? a.width : l.seg) / 4);
+        }
+        if (zeros && zero_weight_grad()) {
+            p.zero[1] = static_cast<uint4*>(a.weight_grad);
+            p.zero_count[1] = static_cast<int64_t>(a.classes * a.width / 4);
+        }
         p.src = src;
         p.src_ld = static_cast<int64_t>(src_ld);
         p.rows = static_cast<int64_t>(rows);
@@ -658,6 +677,22 @@ struct Call {
         else kernel<<<grid, threads, 0, stream>>>(p, vec);
         return launched("vocabulary loss pack kernel launch", err);
     }
+
+    // f32 gradients whose sums are split have to start from zeros, which the hidden rows' packing writes: a memset before
+    // each product takes 2.5 us and keeps the product's set-up from overlapping the kernel before it (1,021 x 256 x 10,007:
+    // 168 us, 163 us this way). Not over hidden rows that the gradient is to replace: they are still being read.
+    bool zero_hidden_grad() const {
+        const auto h = reinterpret_cast<uintptr_t>(a.hidden), g = reinterpret_cast<uintptr_t>(a.hidden_grad);
+        const uint64_t h_bytes = ((a.rows - 1) * a.hidden_stride + a.width) * l.elem, g_bytes = a.rows * a.width * 4;
+        return l.f32 && !deterministic && a.hidden_grad != nullptr && l.piece > kSumLength &&
+               (!l.hidden_grad_direct || g + g_bytes <= h || h + h_bytes <= g);
+    }
+    bool zero_weight_grad() const {
+        return l.f32 && !deterministic && a.weight_grad != nullptr && a.accumulate == 0 && l.weight_grad_direct &&
+               a.rows > kSumLength;
+    }
+
+    void* hidden_sums() const { return l.hidden_grad_direct ? a.hidden_grad : at(l.dh_at); }
 
     const void* hidden() const { return l.pack_hidden ? at(l.hidden_at) : a.hidden; }
 
@@ -796,9 +831,8 @@ struct Call {
     int hidden_grad(uint64_t v0, uint64_t n, const void* w) const {
         const snb_operand left{l.grad_ld, 1, 0};
         const snb_operand right = a.weight_transposed ? snb_operand{l.weight_ld, 1, 0} : snb_operand{1, l.weight_ld, 0};
-        const bool direct = l.hidden_grad_direct;
-        return product(a.rows, direct ? a.width : l.seg, n, grad_part(), left, weight_part(w), right,
-                       direct ? a.hidden_grad : at(l.dh_at), SNB_TYPE_F32, v0 > 0);
+        return product(a.rows, l.hidden_grad_direct ? a.width : l.seg, n, grad_part(), left, weight_part(w), right,
+                       hidden_sums(), SNB_TYPE_F32, v0 > 0 || zero_hidden_grad());
     }
 
     // Whether an output's tiles, unsplit, keep three fifths of the CTA pairs' rounds busy.
@@ -817,9 +851,9 @@ struct Call {
             // The rows of the piece are contiguous in the gradient: written there unless a row is no multiple of 16
             // bytes, or a bf16 gradient has so few tiles that its sums are better split (which needs f32).
             const bool dense = a.width * es % 16 == 0 && aligned16(out);
-            if (dense && (a.weight_grad_type == SNB_TYPE_F32 || fills(n, a.width)))
+            if (l.weight_grad_direct || (dense && a.weight_grad_type == SNB_TYPE_BF16 && fills(n, a.width)))
                 return product(n, a.width, a.rows, grad_part(), p_t, hidden_part(), h, out, a.weight_grad_type,
-                               a.accumulate != 0);
+                               a.accumulate != 0 || zero_weight_grad());
             rc = product(n, l.seg, a.rows, grad_part(), p_t, hidden_part(), h, at(l.dw_at), SNB_TYPE_F32, false);
             return rc != SNB_OK ? rc : store(at(l.dw_at), l.wgrad_ld, out, a.weight_grad_type, a.width, n, a.width,
                                              a.accumulate != 0);
@@ -887,7 +921,7 @@ struct Call {
         constexpr int kLoHiHi = 1;
         if (l.pack_hidden) {
             rc = pack(a.hidden, a.hidden_stride, a.rows, a.width, at(l.hidden_at), l.hidden_ld, a.rows, l.seg,
-                      l.gradients ? a.targets : nullptr, l.seg, kLoHiHi, false);
+                      l.gradients ? a.targets : nullptr, l.seg, kLoHiHi, false, true);
             if (rc != SNB_OK) return rc;
         }
         // Pass 1: a weight that is read in place needs no pieces here.

@@ -94,6 +94,32 @@ def test_losses_and_gradients(rows, width, classes, dtype, storage):
     _check(*_case(rows, width, classes, dtype, storage, seed=rows + classes), storage)
 
 
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("rows,width,classes", [(300, 256, 1003), (40, 99, 513), (513, 64, 200)])
+def test_the_hidden_gradient_may_replace_the_hidden_rows(rows, width, classes, dtype):
+    hidden, weight, targets = _case(rows, width, classes, dtype, Storage.TRANSPOSED, seed=rows)
+    hidden = hidden.contiguous()
+    losses_e, _, _, dh_e, dw_e = _reference(hidden, weight, targets, Storage.TRANSPOSED, 0.5)
+    dw = torch.full(weight.shape, float("nan"), device="cuda", dtype=dtype)
+    losses, _ = _run(hidden, weight, targets, Storage.TRANSPOSED, d_hidden=hidden, d_weight=dw, grad_scale=0.5)
+    _close(losses, losses_e, 1e-5)
+    _close(hidden, dh_e, GRAD_TOLERANCE[dtype])
+    _close(dw, dw_e, GRAD_TOLERANCE[dtype])
+
+
+@pytest.mark.parametrize("offset", [0, 1, 2])
+def test_f32_gradients_that_start_off_16_bytes(offset):
+    hidden, weight, targets = _case(700, 100, 1003, F32, Storage.TRANSPOSED, seed=offset)
+    _, _, _, dh_e, dw_e = _reference(hidden, weight, targets, Storage.TRANSPOSED, 0.5)
+    whole = [torch.full((t.numel() + 8,), float("nan"), device="cuda") for t in (hidden, weight)]
+    dh, dw = (w[offset:offset + t.numel()].view(t.shape) for w, t in zip(whole, (hidden, weight)))
+    _run(hidden, weight, targets, Storage.TRANSPOSED, d_hidden=dh, d_weight=dw, grad_scale=0.5)
+    _close(dh, dh_e, GRAD_TOLERANCE[F32])
+    _close(dw, dw_e, GRAD_TOLERANCE[F32])
+    for w, t in zip(whole, (hidden, weight)):
+        assert bool(w[:offset].isnan().all()) and bool(w[offset + t.numel():].isnan().all())
+
+
 @pytest.mark.parametrize("storage", list(Storage), ids=lambda s: s.name.lower())
 @pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
 @pytest.mark.parametrize("rows", [1, 2, 3, 4, 5, 7, 16, 17])
