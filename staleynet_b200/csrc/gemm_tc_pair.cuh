@@ -243,6 +243,8 @@ __global__ void __cluster_dims__(2, 1, 1) __launch_bounds__(TC_THREADS, 1)
             const TcUnit u0 = tc_cursor_unit(p, cur, BN, BK, TC2_BM);
             request_aux_boxes<OUT_BF16, BN>(p, &tm_aux, u0, u0.m0 + row_off, group, boxes, aux_bar);
         }
+        if constexpr (EPI == TC_EPI_LSE)
+            target_logits<E>(p, blockIdx.x * TC_EPI_WARPS + warp - TC_EPI_WARP0, gridDim.x * TC_EPI_WARPS);
         for (; cur.unit < p.num_units; tc_advance(p, cur)) {
             const TcUnit u = tc_cursor_unit(p, cur, BN, BK, TC2_BM);
             const int acc = iter & 1;

@@ -129,6 +129,12 @@ struct VocabProduct {
     int64_t class_begin;
     float2* partials;
     float* target_logit;
+    // With the statistics: the targets' logits as rounded f32 sums of the operands as the caller has them; or null.
+    float* exact_logit;
+    const void* hidden;
+    const void* weight;
+    uint64_t hidden_row, weight_class, weight_inner, width;  // element strides
+    uint64_t vocabulary;     // classes of the whole
     const float2* row_stats;
     void* grad;
     void* grad_low;

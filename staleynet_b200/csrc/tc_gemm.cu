@@ -719,6 +719,17 @@ int tc_vocab_product(cudaStream_t stream, const VocabProduct& v, std::string* er
     p.class_begin = v.class_begin;
     p.partials = v.partials;
     p.target_logit = v.target_logit;
+    p.hidden = v.hidden;
+    p.weight = v.weight;
+    p.hidden_row = static_cast<int64_t>(v.hidden_row);
+    p.weight_class = static_cast<int64_t>(v.weight_class);
+    p.weight_inner = static_cast<int64_t>(v.weight_inner);
+    p.width = static_cast<int32_t>(v.width);
+    const uint64_t per16 = 16 / esize;
+    p.exact_vec = v.weight_inner == 1 && v.width % per16 == 0 && v.hidden_row % per16 == 0 && v.weight_class % per16 == 0 &&
+                  (reinterpret_cast<uintptr_t>(v.hidden) | reinterpret_cast<uintptr_t>(v.weight)) % 16 == 0;
+    p.classes = static_cast<int64_t>(v.vocabulary);
+    p.exact_logit = v.grad == nullptr ? v.exact_logit : nullptr;
     p.row_stats = v.row_stats;
     const int workers = pair ? sms / 2 : sms;
     const int grid = static_cast<int>(std::min<int64_t>(p.num_units, workers)) * (pair ? 2 : 1);

@@ -197,7 +197,7 @@ __device__ __forceinline__ void join(float2& a, float2 b) {
 // 32,768 (17 MB).
 __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     combine_kernel(const float2* partials, int64_t pairs, int64_t rows, const uint32_t* targets, uint64_t classes,
-                   const float* target_logit, float* losses, float2* row_stats, float* loss_sum) {
+                   const float* target_logit, const float* exact_logit, float* losses, float2* row_stats, float* loss_sum) {
     __shared__ float2 part[kCombineLanes][kCombineRows + 1];
     __shared__ float row_loss[kCombineRows];
     allow_next_kernel();
@@ -205,6 +205,14 @@ __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     const int r = threadIdx.x & 31, w = threadIdx.x >> 5;
     const float inf = __int_as_float(0x7f800000);
     float2 v = make_float2(-inf, 0.0f);
+    const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + w;
+    uint32_t t = kEmptyToken;
+    float z = 0.0f, exact = 0.0f;
+    if (r == 0 && row < rows) {  // (read early: the tree below waits for the pairs anyway)
+        t = targets[row];
+        z = target_logit[row];
+        exact = exact_logit != nullptr ? exact_logit[row] : z;
+    }
     const int64_t read_row = static_cast<int64_t>(blockIdx.x) * kCombineRows + r;
     if (read_row < rows) {
         // Several pairs at a time: their reads overlap, and all but one factor of their sums are independent of each other.
@@ -233,12 +241,14 @@ __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
         const float2 other = make_float2(__shfl_xor_sync(0xffffffffu, v.x, d), __shfl_xor_sync(0xffffffffu, v.y, d));
         join(v, other);
     }
-    const int64_t row = static_cast<int64_t>(blockIdx.x) * kCombineRows + w;
     float loss = 0.0f;
     if (r == 0 && row < rows) {
-        const uint32_t t = targets[row];
         const float nan = __int_as_float(0x7fc00000);
-        if (t != kEmptyToken) loss = t < classes ? (v.x - target_logit[row]) + logf(v.y) : nan;
+        if (t != kEmptyToken) loss = t < classes ? (v.x - z) + logf(v.y) : nan;
+        // The exact logit z + d in the place of z, in the target's term of the sum as well: with p its share exp(-loss),
+        // lse grows by log(1 + p (e^d - 1)). (Not where z or the loss is no number or infinite.)
+        const float d = exact - z;
+        if (t < classes && fabsf(d) < 1.0f && loss < inf) loss += log1pf(expf(-loss) * expm1f(d)) - d;
         losses[row] = loss;
         if (row_stats != nullptr)
             row_stats[row] = t == kEmptyToken ? make_float2(inf, 0.0f)
@@ -508,7 +518,8 @@ struct Layout {
     uint64_t wgrad_ld, wgrad_rows;   // f32 weight gradient of a piece before it is stored
     bool hidden_grad_direct;         // dH is summed where the caller wants it
     bool weight_grad_direct;         // so is dW [classes, width]
-    uint64_t hidden_at, weight_at, partials_at, target_at, stats_at, p_at, dh_at, dw_at, bytes;
+    bool exact;                      // the targets' logits are computed once more (target_logits)
+    uint64_t hidden_at, weight_at, partials_at, target_at, exact_at, stats_at, p_at, dh_at, dw_at, bytes;
 };
 
 bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0; }
@@ -586,7 +597,13 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     l.weight_at = take(l.pack_weight ? (a.weight_transposed ? l.piece * l.weight_ld
                                                             : (l.f32 ? 3 : 1) * l.seg * l.weight_ld) * l.elem : 0);
     l.partials_at = take((l.few ? l.few_blocks : (a.classes + kHalfTile - 1) / kHalfTile) * a.rows * sizeof(float2));
+    // (The tensor cores wait for the epilogue warps meanwhile, and their waits are bounded: this keeps it to milliseconds.)
+    // Not for many rows of bf16 over a weight [width, classes], whose columns are gathered element by element (8,192 x 768 x
+    // 32,768: 33 us of 1,416) for losses that are 4e-7 off without.
+    l.exact = !l.few && a.rows * a.width <= (1ull << 31) &&
+              (l.f32 || a.weight_transposed != 0 || a.rows <= 16 * static_cast<uint64_t>(sms));
     l.target_at = take(a.rows * 4);
+    l.exact_at = take(l.exact ? a.rows * 4 : 0);
     l.stats_at = take(a.rows * sizeof(float2));
     l.p_at = take(l.gradients ? a.rows * l.grad_ld * (l.f32 ? 8 : 2) : 0);
     l.dh_at = take(a.hidden_grad != nullptr && !l.hidden_grad_direct ? a.rows * l.seg * 4 : 0);
@@ -694,6 +711,8 @@ struct Call {
 
     void* hidden_sums() const { return l.hidden_grad_direct ? a.hidden_grad : at(l.dh_at); }
 
+    float* exact_logit() const { return l.exact ? static_cast<float*>(at(l.exact_at)) : nullptr; }
+
     const void* hidden() const { return l.pack_hidden ? at(l.hidden_at) : a.hidden; }
 
     Part hidden_part() const {
@@ -742,6 +761,14 @@ struct Call {
         v.class_begin = static_cast<int64_t>(v0);
         v.partials = static_cast<float2*>(at(l.partials_at)) + v0 / kHalfTile * a.rows;
         v.target_logit = static_cast<float*>(at(l.target_at));
+        v.exact_logit = v0 == 0 ? exact_logit() : nullptr;
+        v.vocabulary = a.classes;
+        v.hidden = a.hidden;
+        v.weight = a.weight;
+        v.hidden_row = a.hidden_stride;
+        v.weight_class = a.weight_transposed ? a.weight_stride : 1;
+        v.weight_inner = a.weight_transposed ? 1 : a.weight_stride;
+        v.width = a.width;
         v.row_stats = static_cast<const float2*>(at(l.stats_at));
         v.sm_budget = sm_budget;
         return v;
@@ -936,7 +963,7 @@ struct Call {
         const uint64_t blocks = (a.rows + kCombineRows - 1) / kCombineRows;
         launch_early(combine_kernel, static_cast<unsigned>(blocks), kCombineRows * kCombineLanes, stream,
                      static_cast<const float2*>(at(l.partials_at)), l.few ? l.few_blocks : (a.classes + kHalfTile - 1) / kHalfTile, a.rows, a.targets,
-                     a.classes, static_cast<const float*>(at(l.target_at)), a.losses,
+                     a.classes, static_cast<const float*>(at(l.target_at)), exact_logit(), a.losses,
                      l.gradients ? static_cast<float2*>(at(l.stats_at)) : nullptr, a.loss_sum);
         if ((rc = launched("combine_kernel launch", err)) != SNB_OK) return rc;
         if (a.loss_sum != nullptr && blocks > 1) {

@@ -107,6 +107,30 @@ def test_the_hidden_gradient_may_replace_the_hidden_rows(rows, width, classes, d
     _close(dw, dw_e, GRAD_TOLERANCE[dtype])
 
 
+@pytest.mark.parametrize("storage", list(Storage), ids=lambda s: s.name.lower())
+@pytest.mark.parametrize("dtype", [F32, BF16], ids=["f32", "bf16"])
+@pytest.mark.parametrize("width", [1024, 1003])
+def test_a_target_far_from_zero_costs_no_accuracy(width, dtype, storage):
+    """A matrix instruction (8 products of f32 operands, 16 of bf16) loses up to 2^-24 of its sum towards zero. That may show
+    in the other classes' logits, weighted with their shares, but not in a target's logit, which is several times larger."""
+    rows, classes = 300, 20011
+    g = torch.Generator(device="cuda").manual_seed(width)
+    w = torch.randn(classes, width, generator=g, device="cuda") * width ** -0.5
+    targets = torch.randint(0, classes, (rows,), generator=g, device="cuda", dtype=torch.int32)
+    hidden = (torch.randn(rows, width, generator=g, device="cuda") + 9.0 * w[targets.long()]).to(dtype)
+    weight = (w if storage is Storage.TRANSPOSED else w.t().contiguous()).to(dtype)
+    losses_e, lse, *_ = _reference(hidden, weight, targets, storage, 1.0)
+    z = hidden.double() @ (weight.double().t() if storage is Storage.TRANSPOSED else weight.double())
+    at = targets.long()[:, None]
+    share = torch.exp(z - lse[:, None]).scatter_(1, at, 0.0)
+    instructions = width / (8 if dtype == F32 else 16)
+    bound = instructions * 2.0 ** -24 * (share * z.abs()).sum(1) + 4 * 2.0 ** -24 * (lse.abs() + z.gather(1, at)[:, 0].abs())
+    dh = torch.empty_like(hidden)
+    for more in ({}, {"d_hidden": dh}):
+        losses, _ = _run(hidden, weight, targets, storage, **more)
+        assert (losses.double() - losses_e).abs().mean() <= bound.mean()
+
+
 @pytest.mark.parametrize("offset", [0, 1, 2])
 def test_f32_gradients_that_start_off_16_bytes(offset):
     hidden, weight, targets = _case(700, 100, 1003, F32, Storage.TRANSPOSED, seed=offset)
