@@ -168,7 +168,7 @@ __device__ __forceinline__ TcUnit tc_make_unit(const TcParams& p, int32_t split,
         const int64_t first_query = static_cast<int64_t>(u.m0) - p.causal_offset;
         if (first_query > 0) u.kb_begin = max(u.kb_begin, static_cast<int32_t>(first_query / BK));
     }
-    if (p.two_planes) {
+    if (BK == 128 / 4 && p.two_planes) {  // (f32 slices: the bf16 kernels, whose BK is another constant, leave this out)
         const int64_t low = 2 * static_cast<int64_t>(p.k_blocks);
         u.low_begin = static_cast<int32_t>(u.split * low / p.splits);
         u.low_slices = static_cast<int32_t>((u.split + 1) * low / p.splits) - u.low_begin;
