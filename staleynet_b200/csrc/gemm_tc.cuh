@@ -604,7 +604,8 @@ __device__ __forceinline__ void epilogue_tile(const TcParams& p, const CUtensorM
 // row's running maximum and sum in its lane's registers: when a later 32-column piece raises the maximum from m to m',
 // the sum is multiplied by 2^(m - m'). One (maximum, sum) pair for each row and half tile goes to `partials`, so the
 // halves are joined in a fixed order by a later kernel, without atomics. The exponents are always taken against the
-// rounded product k * max, so its rounding cancels and large logits cost no more accuracy than their own rounding.
+// rounded product k * max, and so are the loss and the gradient that follow: its rounding cancels, and large logits cost no
+// more accuracy than their own rounding.
 template <int BN>
 __device__ __forceinline__ void lse_tile(const TcParams& p, const TcUnit& u, int32_t row0, uint32_t t_lane, int group) {
     constexpr float kLog2eTile = 1.4426950408889634f;

@@ -38,7 +38,7 @@ constexpr uint64_t kWeightBytes = 256ull << 20;    // bound of a packed piece of
 // products) instead of rounding: 2^-24 of the sum each time on average, always towards zero. Measured as the relative
 // error of a weight gradient over 1,021 rows: 2.5e-6 in one sum, 0.7e-6 in sums of 256 (0.6e-6 with f32 arithmetic).
 constexpr uint64_t kSumLength = 256;
-constexpr float kLog2e = 1.4426950408889634f;
+constexpr float kLog2e = 1.4426950408889634f, kLn2 = 0.6931471805599453f;
 constexpr uint64_t kHalfTile = 128;                // classes that one (maximum, sum) pair covers
 
 __device__ __forceinline__ uint16_t bf16_bits(float f) {
@@ -244,11 +244,16 @@ __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
     float loss = 0.0f;
     if (r == 0 && row < rows) {
         const float nan = __int_as_float(0x7fc00000);
-        if (t != kEmptyToken) loss = t < classes ? (v.x - z) + logf(v.y) : nan;
+        // The sum is one of exponentials above the rounded product `base`, so lse = ln 2 (base + log2 sum): taken against the
+        // maximum itself, each loss would be off by base's rounding (up to 1e-5 for logits of 200). The fused difference of
+        // base and k z rounds once more, after the two have cancelled.
+        const float base = __fmul_rn(v.x, kLog2e);
+        if (t != kEmptyToken) loss = t < classes ? kLn2 * (fmaf(-z, kLog2e, base) + log2f(v.y)) : nan;
         // The exact logit z + d in the place of z, in the target's term of the sum as well: with p its share exp(-loss),
         // lse grows by log(1 + p (e^d - 1)). (Not where z or the loss is no number or infinite.)
         const float d = exact - z;
         if (t < classes && fabsf(d) < 1.0f && loss < inf) loss += log1pf(expf(-loss) * expm1f(d)) - d;
+        if (loss < 0.0f) loss = 0.0f;  // what is left of the roundings of a loss of 0
         losses[row] = loss;
         if (row_stats != nullptr)
             row_stats[row] = t == kEmptyToken ? make_float2(inf, 0.0f)
