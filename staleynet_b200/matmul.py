@@ -580,8 +580,10 @@ class Gpu:
         a = self._vocabulary_loss_args(hidden, weight, storage, d_hidden, d_weight)
         if targets.dtype != torch.int32 or not targets.is_contiguous():
             raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: targets must be dense int32")
-        if losses.dtype != torch.float32 or (loss_sum is not None and loss_sum.dtype != torch.float32):
-            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: losses must be float32")
+        if losses.dtype != torch.float32 or not losses.is_contiguous():
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: losses must be dense float32")
+        if loss_sum is not None and (loss_sum.dtype != torch.float32 or loss_sum.numel() != 1):
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: loss_sum must be one float32")
         a.targets, a.targets_len = targets.data_ptr(), targets.numel()
         a.losses, a.losses_len = losses.data_ptr(), losses.numel()
         a.loss_sum = loss_sum.data_ptr() if loss_sum is not None else None
