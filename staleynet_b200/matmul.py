@@ -384,7 +384,7 @@ class Gpu:
                 or input_grad.dtype is not input.dtype or gain.dtype is not f32 or mean.dtype is not f32
                 or inv_std.dtype is not f32 or gain_grad.dtype is not f32 or not input.is_cuda or not output_grad.is_cuda
                 or not input_grad.is_cuda or not gain.is_cuda or not mean.is_cuda or not inv_std.is_cuda
-                or not gain_grad.is_cuda or not workspace.is_cuda or not gain.is_contiguous()
+                or not gain_grad.is_cuda or not workspace.is_cuda or not workspace.is_contiguous() or not gain.is_contiguous()
                 or not mean.is_contiguous() or not inv_std.is_contiguous() or not gain_grad.is_contiguous()
                 or (bias_grad is not None
                     and (bias_grad.dtype is not f32 or not bias_grad.is_cuda or not bias_grad.is_contiguous()))
@@ -393,6 +393,8 @@ class Gpu:
                               {"input": input, "output_grad": output_grad, "input_grad": input_grad},
                               (gain, gain_grad) if bias_grad is None else (gain, gain_grad, bias_grad), (mean, inv_std))
             _require_cuda(workspace)
+            if not workspace.is_contiguous():
+                raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "layer_norm_backward: workspace must be dense")
             raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "layer_norm_backward: input_grad must have the input's dtype")
         rows, cols = shape
         many = rows > 1
@@ -580,6 +582,8 @@ class Gpu:
         a = self._vocabulary_loss_args(hidden, weight, storage, d_hidden, d_weight)
         if targets.dtype != torch.int32 or not targets.is_contiguous():
             raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: targets must be dense int32")
+        if not workspace.is_contiguous():
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: workspace must be dense")
         if losses.dtype != torch.float32 or not losses.is_contiguous():
             raise SnbError(_ffi.ERR_INVALID_ARGUMENT, "vocabulary_cross_entropy: losses must be dense float32")
         if loss_sum is not None and (loss_sum.dtype != torch.float32 or loss_sum.numel() != 1):

@@ -56,3 +56,14 @@ def test_the_losses_are_dense(losses):
 def test_the_sum_of_the_losses_is_one_f32(total):
     with pytest.raises(SnbError, match="loss_sum must be one float32"):
         _loss(loss_sum=total)
+
+
+@pytest.mark.parametrize("workspace", [torch.zeros(8192, dtype=torch.uint8)[::2],
+                                       torch.zeros(1, dtype=torch.uint8).expand(4096)], ids=["strided", "expanded"])
+def test_the_workspace_is_dense(workspace):
+    with pytest.raises(SnbError, match="vocabulary_cross_entropy: workspace must be dense"):
+        _loss(workspace=workspace)
+    rows, params, stats = (torch.zeros(6, 40) for _ in range(3)), (torch.zeros(40) for _ in range(3)), torch.zeros(6)
+    (dy, x, dx), (gain, dg, db) = rows, params
+    with pytest.raises(SnbError, match="layer_norm_backward: workspace must be dense"):
+        _gpu().layer_norm_backward(*(_on_device(t) for t in (dy, x, gain, stats, stats, dx, dg, db, workspace)))
