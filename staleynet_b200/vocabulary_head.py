@@ -39,9 +39,12 @@ class VocabularyHead:
         self.mean, self.inv_std, self.losses, self.loss_sum = empty(rows), empty(rows), empty(rows), empty(())
         self.d_weight = torch.empty_like(self.operand)
         self.d_gain, self.d_bias = torch.empty_like(self.gain), torch.empty_like(self.bias)
-        need = gpu.vocabulary_cross_entropy_workspace(self.normal, self.operand, d_hidden=self.d_normal,
-                                                      d_weight=self.d_weight)
-        self.workspace = empty(max(need, gpu.layer_norm_workspace(rows, width)), dtype=torch.uint8)
+        # For evaluate and for backward: either may need more (the loss alone packs longer pieces of an f32 weight).
+        need = max(gpu.vocabulary_cross_entropy_workspace(self.normal, self.operand),
+                   gpu.vocabulary_cross_entropy_workspace(self.normal, self.operand, d_hidden=self.d_normal,
+                                                          d_weight=self.d_weight),
+                   gpu.layer_norm_workspace(rows, width))
+        self.workspace = empty(need, dtype=torch.uint8)
         self.optimizer = AdamW8(gpu, [
             AdamW8Tensor(self.weight, self.d_weight, *adamw8_state(self.weight), weight_decay=weight_decay,
                          shadow=self.operand if bf16 else None),
