@@ -273,6 +273,7 @@ __global__ void __launch_bounds__(kCombineRows * kCombineLanes)
 // in one pass over the weight, which is what bounds it, on the CUDA cores. Logits are f32 sums; each thread block leaves one
 // (maximum, sum) pair for each row.
 constexpr int kFewThreads = 256;
+constexpr uint64_t kFewWidth = 4096;  // longest hidden row: four as f32 take 64 KB of shared memory
 
 struct FewParams {
     const void* hidden;
@@ -538,7 +539,7 @@ bool few_rows(const snb_vocabulary_loss_args& a) {
     const uint64_t per16 = a.type == SNB_TYPE_BF16 ? 8 : 4;
     const bool readable = a.type == SNB_TYPE_BF16 && aligned16(a.weight) && a.weight_stride % per16 == 0;
     return a.hidden_grad == nullptr && a.weight_grad == nullptr && !readable &&
-           a.rows <= (a.type == SNB_TYPE_BF16 ? 4 : 16) && a.width <= 4096;
+           a.rows <= (a.type == SNB_TYPE_BF16 ? 4 : 16) && a.width <= kFewWidth;
 }
 
 Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
@@ -906,11 +907,16 @@ struct Call {
 
     template <int R, typename E>
     int few_typed(const FewParams& p) const {
-        int64_t smem = 4ll * R * (a.weight_transposed ? (p.width + 255) & ~255 : p.width);
-        if (!a.weight_transposed) smem = (smem + 15) / 16 * 16 + 4ll * kFewThreads * R * (16 / static_cast<int>(sizeof(E)));
+        const auto shared = [&](int64_t width) -> int64_t {
+            if (a.weight_transposed) return 4ll * R * ((width + 255) & ~255ll);
+            return (4ll * R * width + 15) / 16 * 16 + 4ll * kFewThreads * R * (16 / static_cast<int>(sizeof(E)));
+        };
+        const int64_t smem = shared(p.width), most = shared(kFewWidth);
         const auto kernel = a.weight_transposed ? few_rows_kernel<R, E> : few_rows_across_kernel<R, E>;
-        if (smem > (44 << 10)) {
-            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem));
+        // What the kernel may use is a setting of the kernel, not of the launch: always the same one, or a call of another
+        // thread could lower it between this call's setting and its launch.
+        if (most > (44 << 10)) {
+            const cudaError_t e = cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(most));
             if (e != cudaSuccess) {
                 *err = cuda_message("cudaFuncSetAttribute(few_rows_kernel)", e);
                 return SNB_ERR_CUDA;
