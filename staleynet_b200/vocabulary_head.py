@@ -12,12 +12,13 @@ from __future__ import annotations
 
 import argparse
 
+from . import _ffi
 from .adamw8 import AdamW8, AdamW8Tensor, adamw8_state
-from .matmul import AdamWHyperparameters, DeviceRandom, Gpu, Storage
+from .matmul import AdamWHyperparameters, DeviceRandom, Gpu, SnbError, Storage
 
 
 class VocabularyHead:
-    """Weights, optimizer state and buffers of the layer for micro-batches of `rows` tokens. The weight is
+    """Weights, optimizer state and buffers of the layer for micro-batches of up to `rows` tokens. The weight is
     [classes, width] (a tied embedding's layout); `dtype` is the activations' and their gradients' element type."""
 
     def __init__(self, gpu: Gpu, rows: int, width: int, classes: int, seed: int = 1, weight_decay: float = 0.1,
@@ -52,31 +53,55 @@ class VocabularyHead:
             AdamW8Tensor(self.bias, self.d_bias, *adamw8_state(self.bias)),
         ])
 
+    def _rows_of(self, hidden, *buffers):
+        """The first rows of buffers for the rows of a batch, of which there may be fewer than the layer's."""
+        n = hidden.shape[0]
+        if n == self.rows:
+            return buffers
+        if n > self.rows:
+            raise SnbError(_ffi.ERR_INVALID_ARGUMENT, f"vocabulary head: {n} rows, made for at most {self.rows}")
+        return tuple(b[:n] for b in buffers)
+
+    def _workspace_of(self, normal, **gradients):
+        """A workspace for the loss of these rows. Fewer rows may need more (their pieces are longer): it grows then."""
+        if normal is not self.normal:
+            need = self.gpu.vocabulary_cross_entropy_workspace(normal, self.operand, **gradients)
+            if need > self.workspace.numel():
+                import torch
+
+                with torch.cuda.stream(self.gpu.stream):   # (the old one goes back to the stream that may still use it)
+                    self.workspace = self.workspace.new_empty(need)
+        return self.workspace
+
     def evaluate(self, hidden, targets):
-        """The rows' losses (0 where the target is -1), without gradients; `loss_sum` receives their sum."""
-        self.gpu.layer_norm_forward(hidden, self.gain, self.bias, self.normal, self.mean, self.inv_std, self.epsilon)
-        self.gpu.vocabulary_cross_entropy(self.normal, self.operand, targets, self.losses, self.loss_sum,
-                                          self.workspace, storage=Storage.TRANSPOSED)
-        return self.losses
+        """The rows' losses (0 where the target is -1), without gradients; `loss_sum` receives their sum. Any number of rows
+        up to the layer's; the result is overwritten by the next call."""
+        normal, mean, inv_std, losses = self._rows_of(hidden, self.normal, self.mean, self.inv_std, self.losses)
+        self.gpu.layer_norm_forward(hidden, self.gain, self.bias, normal, mean, inv_std, self.epsilon)
+        self.gpu.vocabulary_cross_entropy(normal, self.operand, targets, losses, self.loss_sum,
+                                          self._workspace_of(normal), storage=Storage.TRANSPOSED)
+        return losses
 
     def backward(self, hidden, targets, grad_scale: float):
         """Losses and gradients, times grad_scale: of hidden (returned), and of the weight, gain and bias (d_weight,
-        d_gain, d_bias)."""
+        d_gain, d_bias). Any number of rows up to the layer's."""
         gpu = self.gpu
-        gpu.layer_norm_forward(hidden, self.gain, self.bias, self.normal, self.mean, self.inv_std, self.epsilon)
-        gpu.vocabulary_cross_entropy(self.normal, self.operand, targets, self.losses, self.loss_sum, self.workspace,
-                                     storage=Storage.TRANSPOSED, d_hidden=self.d_normal, d_weight=self.d_weight,
+        normal, mean, inv_std, losses, d_normal, d_hidden = self._rows_of(
+            hidden, self.normal, self.mean, self.inv_std, self.losses, self.d_normal, self.d_hidden)
+        workspace = self._workspace_of(normal, d_hidden=d_normal, d_weight=self.d_weight)
+        gpu.layer_norm_forward(hidden, self.gain, self.bias, normal, mean, inv_std, self.epsilon)
+        gpu.vocabulary_cross_entropy(normal, self.operand, targets, losses, self.loss_sum, workspace,
+                                     storage=Storage.TRANSPOSED, d_hidden=d_normal, d_weight=self.d_weight,
                                      grad_scale=grad_scale)
-        gpu.layer_norm_backward(self.d_normal, hidden, self.gain, self.mean, self.inv_std, self.d_hidden, self.d_gain,
-                                self.d_bias, self.workspace)
-        return self.d_hidden
+        gpu.layer_norm_backward(d_normal, hidden, self.gain, mean, inv_std, d_hidden, self.d_gain, self.d_bias, workspace)
+        return d_hidden
 
     def step(self, hidden, targets, hyper: AdamWHyperparameters, max_gradient_norm: float = 1.0,
              grad_scale: float | None = None):
         """One training step on hidden [rows, width] (of the layer's dtype) and targets [rows] int32; returns the
         gradient of hidden. grad_scale: 1 / rows unless given (a caller whose rows miss targets gives one over those
-        that have one)."""
-        d_hidden = self.backward(hidden, targets, 1.0 / self.rows if grad_scale is None else grad_scale)
+        that have one). A batch may have fewer rows than the layer; no rows at all leave the losses' gradients 0."""
+        d_hidden = self.backward(hidden, targets, 1.0 / max(1, len(hidden)) if grad_scale is None else grad_scale)
         self.optimizer.step(hyper, max_gradient_norm, (self.seed << 32) + hyper.step)
         return d_hidden
 
