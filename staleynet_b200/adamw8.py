@@ -80,9 +80,11 @@ class AdamW8:
             a.count, a.first_draw, a.weight_decay = n, first_draw, t.weight_decay
             a.gradient_type = _ffi.TYPE_BF16 if t.gradient.dtype == torch.bfloat16 else _ffi.TYPE_F32
         device = gpu.device
-        self.gradient_square_sum = torch.zeros((), device=device, dtype=torch.float64)
         need = gpu.lib.snb_adamw8_workspace(len(self.tensors))
-        self._workspace = torch.empty(need, device=device, dtype=torch.uint8)
+        # Made on the stream that the steps run on, whichever is current: a zero written later would overwrite a step's sum.
+        with torch.cuda.stream(gpu.stream):
+            self.gradient_square_sum = torch.zeros((), device=device, dtype=torch.float64)
+            self._workspace = torch.empty(need, device=device, dtype=torch.uint8)
         self._out = None
 
     def step(self, hyper: AdamWHyperparameters, max_gradient_norm: float, seed: int) -> None:
