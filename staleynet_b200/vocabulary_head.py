@@ -26,7 +26,14 @@ class VocabularyHead:
         import torch
 
         self.gpu, self.rows, self.epsilon, self.seed = gpu, rows, epsilon, seed
-        dtype = torch.bfloat16 if dtype is None else dtype
+        # On the stream that the calls run on, whichever is current: the tensors' first values are ready for them.
+        with torch.cuda.stream(gpu.stream):
+            self._allocate(width, classes, weight_decay, torch.bfloat16 if dtype is None else dtype)
+
+    def _allocate(self, width, classes, weight_decay, dtype):
+        import torch
+
+        gpu, rows, seed = self.gpu, self.rows, self.seed
 
         def empty(*shape, dtype=torch.float32):
             return torch.empty(*shape, device=gpu.device, dtype=dtype)
