@@ -285,7 +285,7 @@ struct FewParams {
     const uint32_t* targets;
     float2* partials;               // [blocks, all_rows], from this launch's first row on
     float* target_logit;
-    int32_t vec;  // 16-byte accesses to the weight's rows
+    int32_t vec;  // f32: 16-byte accesses to the weight's rows (bf16 rows that allow them are the tensor cores')
 };
 
 __device__ __forceinline__ float element_of(const float* p, int64_t i) { return p[i]; }
@@ -293,28 +293,13 @@ __device__ __forceinline__ float element_of(const uint16_t* p, int64_t i) {
     return __uint_as_float(static_cast<uint32_t>(p[i]) << 16);
 }
 
-// 16 bytes of a row as floats: 4 of f32, 8 of bf16.
-__device__ __forceinline__ void unpack(uint4 q, float (&v)[4]) {
-    v[0] = __uint_as_float(q.x); v[1] = __uint_as_float(q.y); v[2] = __uint_as_float(q.z); v[3] = __uint_as_float(q.w);
-}
-__device__ __forceinline__ void unpack(uint4 q, float (&v)[8]) {
-    const uint32_t w[4] = {q.x, q.y, q.z, q.w};
-#pragma unroll
-    for (int k = 0; k < 4; ++k) {
-        v[2 * k] = __uint_as_float(w[k] << 16);
-        v[2 * k + 1] = __uint_as_float(w[k] & 0xFFFF0000u);
-    }
-}
-
-// The hidden rows as f32 in shared memory, [R, ld], zero past the call's rows. LANES: in the order in which few_rows_kernel
-// reads bf16 weights, where a lane has 8 consecutive elements of each 256: the first halves of all lanes, then the second.
-template <int R, bool LANES, typename E>
+// The hidden rows as f32 in shared memory, [R, ld], zero past the call's rows.
+template <int R, typename E>
 __device__ __forceinline__ void stage_hidden(const FewParams& p, float* h, int ld) {
     for (int k = threadIdx.x; k < p.width; k += kFewThreads) {
-        const int at = LANES ? (k & ~255) + ((k & 4) << 5) + ((k & 0xF8) >> 1) + (k & 3) : k;
 #pragma unroll
         for (int r = 0; r < R; ++r)
-            h[r * ld + at] = r < p.rows ? element_of(static_cast<const E*>(p.hidden), r * p.hidden_ld + k) : 0.0f;
+            h[r * ld + k] = r < p.rows ? element_of(static_cast<const E*>(p.hidden), r * p.hidden_ld + k) : 0.0f;
     }
     __syncthreads();
 }
@@ -354,15 +339,13 @@ __device__ __forceinline__ void leave_pairs(const FewParams& p, const float2 (&s
     }
 }
 
-// Weight [classes, width]: a warp takes four classes at a time, its lanes 16 bytes of each row in turn.
+// Weight [classes, width]: a warp takes four classes at a time, its lanes 16 bytes of each f32 row in turn, or an element.
 template <int R, typename E>
 __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p) {
     extern __shared__ __align__(16) float h[];
     allow_next_kernel();
-    constexpr int PER = 16 / sizeof(E);
-    const int ld = (p.width + 255) & ~255;
-    if (PER == 8 && p.vec) stage_hidden<R, true, E>(p, h, ld);
-    else stage_hidden<R, false, E>(p, h, ld);
+    const int ld = (p.width + 3) & ~3;
+    stage_hidden<R, E>(p, h, ld);
     const int lane = threadIdx.x & 31;
     const int64_t warp = static_cast<int64_t>(blockIdx.x) * (kFewThreads / 32) + (threadIdx.x >> 5);
     const int64_t warps = static_cast<int64_t>(gridDim.x) * (kFewThreads / 32);
@@ -376,32 +359,27 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_kernel(const FewParams p
 #pragma unroll
         for (int r = 0; r < R; ++r) z[r][0] = z[r][1] = z[r][2] = z[r][3] = 0.0f;
         const E* rows = weight + v0 * p.weight_ld;
-        if (p.vec) {
+        bool done = false;
+        if constexpr (sizeof(E) == 4) {
+            if (p.vec) {
+                done = true;
 #pragma unroll 3
-            for (int k = lane * PER; k < p.width; k += 32 * PER) {
-                uint4 q[4];
+                for (int k = lane * 4; k < p.width; k += 32 * 4) {
+                    float4 q[4];
 #pragma unroll
-                for (int c = 0; c < 4; ++c)
-                    q[c] = c < n ? __ldg(reinterpret_cast<const uint4*>(rows + c * p.weight_ld + k)) : make_uint4(0, 0, 0, 0);
+                    for (int c = 0; c < 4; ++c)
+                        q[c] = c < n ? __ldg(reinterpret_cast<const float4*>(rows + c * p.weight_ld + k)) : make_float4(0, 0, 0, 0);
 #pragma unroll
-                for (int r = 0; r < R; ++r) {
-                    const float* hr = h + r * ld + (PER == 8 ? (k & ~255) + 4 * lane : k);
-                    float x[PER];
+                    for (int r = 0; r < R; ++r) {
+                        const float4 x = *reinterpret_cast<const float4*>(h + r * ld + k);
 #pragma unroll
-                    for (int e = 0; e < PER; e += 4) {
-                        const float4 f = *reinterpret_cast<const float4*>(hr + 32 * e);
-                        x[e] = f.x; x[e + 1] = f.y; x[e + 2] = f.z; x[e + 3] = f.w;
-                    }
-#pragma unroll
-                    for (int c = 0; c < 4; ++c) {
-                        float w[PER];
-                        unpack(q[c], w);
-#pragma unroll
-                        for (int e = 0; e < PER; ++e) z[r][c] = fmaf(w[e], x[e], z[r][c]);
+                        for (int c = 0; c < 4; ++c)
+                            z[r][c] = fmaf(q[c].w, x.w, fmaf(q[c].z, x.z, fmaf(q[c].y, x.y, fmaf(q[c].x, x.x, z[r][c]))));
                     }
                 }
             }
-        } else {
+        }
+        if (!done) {
             for (int k = lane; k < p.width; k += 32)
                 for (int c = 0; c < n; ++c) {
                     const float w = element_of(rows, c * p.weight_ld + k);
@@ -433,7 +411,7 @@ template <int R, typename E>
 __global__ void __launch_bounds__(kFewThreads) few_rows_across_kernel(const FewParams p) {
     extern __shared__ __align__(16) float h[];  // [R, width], then [8 warps, R, 32 PER] sums
     allow_next_kernel();
-    stage_hidden<R, false, E>(p, h, p.width);
+    stage_hidden<R, E>(p, h, p.width);
     constexpr int PER = 16 / sizeof(E);
     constexpr int WARPS = kFewThreads / 32;
     float* sums = h + (R * p.width + 3) / 4 * 4;
@@ -448,13 +426,16 @@ __global__ void __launch_bounds__(kFewThreads) few_rows_across_kernel(const FewP
         for (int e = 0; e < PER; ++e) z[r][e] = 0.0f;
     const int each = (p.width + WARPS - 1) / WARPS;
     const int end = min(p.width, (w + 1) * each);
-    const bool whole = p.vec && v + PER <= p.classes;
+    const bool whole = sizeof(E) == 4 && p.vec && v + PER <= p.classes;
 #pragma unroll 8
     for (int k = w * each; k < end; ++k) {
         const E* row = weight + static_cast<int64_t>(k) * p.weight_ld + v;
         float x[PER];
         if (whole) {
-            unpack(__ldg(reinterpret_cast<const uint4*>(row)), x);
+            if constexpr (sizeof(E) == 4) {
+                const float4 q = __ldg(reinterpret_cast<const float4*>(row));
+                x[0] = q.x; x[1] = q.y; x[2] = q.z; x[3] = q.w;
+            }
         } else {
 #pragma unroll
             for (int e = 0; e < PER; ++e) x[e] = v + e < p.classes ? element_of(row, e) : 0.0f;
@@ -908,7 +889,7 @@ struct Call {
     template <int R, typename E>
     int few_typed(const FewParams& p) const {
         const auto shared = [&](int64_t width) -> int64_t {
-            if (a.weight_transposed) return 4ll * R * ((width + 255) & ~255ll);
+            if (a.weight_transposed) return 4ll * R * ((width + 3) & ~3ll);
             return (4ll * R * width + 15) / 16 * 16 + 4ll * kFewThreads * R * (16 / static_cast<int>(sizeof(E)));
         };
         const int64_t smem = shared(p.width), most = shared(kFewWidth);
@@ -938,8 +919,7 @@ struct Call {
         p.targets = a.targets;
         p.partials = static_cast<float2*>(at(l.partials_at));
         p.target_logit = static_cast<float*>(at(l.target_at));
-        const uint64_t per16 = 16 / l.elem;
-        p.vec = aligned16(a.weight) && a.weight_stride % per16 == 0 && (!a.weight_transposed || a.width % per16 == 0);
+        p.vec = l.f32 && aligned16(a.weight) && a.weight_stride % 4 == 0 && (!a.weight_transposed || a.width % 4 == 0);
         for (uint64_t row = 0; row < a.rows; row += 4) {
             p.rows = static_cast<int32_t>(std::min<uint64_t>(4, a.rows - row));
             int rc;
