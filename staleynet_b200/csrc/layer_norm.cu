@@ -379,6 +379,13 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T == 32 ? 2
     }
 }
 
+// With 24 elements a thread the gain's registers would be the ones too many in the backward pass: the threads read it from
+// shared memory, a copy in their order.
+template <int NE>
+constexpr bool kSharedGain = NE >= 24;
+
+constexpr int64_t kPartBytes = 2 * 32 * sizeof(float2);  // of row_sum2
+
 // Elements past the row's end are zeros in dy and the gain, so they add nothing to any sum.
 template <int T, int NE, int G, bool XB, bool DB>
 __global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T <= 256 ? 2 : 1)
@@ -429,12 +436,9 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T <= 256 ? 
     };
     for (int k = 0; k < (G > 1 ? p.depth - 1 : 1); ++k) request();
     statistics(first);
-    // With 24 elements a thread the gain's registers would be the ones too many: a warp's share a copy, in the order in
-    // which the threads read it.
-    constexpr bool kSharedGain = NE >= 24;
-    __shared__ float4 shared_gain[kSharedGain ? NE / 4 : 1][T];
+    __shared__ float4 shared_gain[kSharedGain<NE> ? NE / 4 : 1][T];
     float2 gain[NE / 2], dg[NE / 2], db[NE / 2];
-    if constexpr (kSharedGain) {
+    if constexpr (kSharedGain<NE>) {
         load_params<T, NE, G>(p.gain, t, cols, gain);
         if (T > 32 || warp == 0) {
 #pragma unroll
@@ -468,7 +472,7 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T <= 256 ? 
         if (++out == p.depth) out = 0;
         // d = dy g of one pair of elements.
         auto gained = [&](float2 o, int k) {
-            if constexpr (kSharedGain) {
+            if constexpr (kSharedGain<NE>) {
                 const float4 g = shared_gain[k / 2][t];
                 return __fmul2_rn(o, k & 1 ? make_float2(g.z, g.w) : make_float2(g.x, g.y));
             } else {
@@ -490,7 +494,7 @@ __global__ void __launch_bounds__(T == 32 ? 32 * kWarpsPerBlock : T, T <= 256 ? 
         }
         const float2 s = row_sum2<T>(make_float2(sum.x + sum.y, product.x + product.y), part, turn);
         const float mean_d = s.x * per_column, mean_dn = s.y * per_column;
-        if constexpr (kSharedGain) {
+        if constexpr (kSharedGain<NE>) {
             // Held until here the row would not fit beside the column sums: it is read from shared memory again.
             read_row<T, NE, G, XB>(x_here, here, t, cols, n);
             read_row<T, NE, G, DB>(dy_here, here + x_slot, t, cols, d);
@@ -688,18 +692,17 @@ int launched(const char* what, std::string* err) {
     return SNB_ERR_CUDA;
 }
 
-// Launches `kernel` with a ring of its own size. Above 48 KB together with the kernel's static shared memory (4 KB at
-// most) that has to be allowed first, a setting of the kernel on its device that is made again when either changes.
+// Launches `kernel` with a ring of shared memory, always of the same size. Above 48 KB together with the kernel's `fixed`
+// bytes that has to be allowed first, once on each device.
 template <auto kernel>
-void launch_ring(unsigned grid, int threads, int64_t smem, cudaStream_t s, const NormParams& p) {
-    static std::atomic<int64_t> allowed{-1};  // device << 32 | bytes
-    if (smem > (44 << 10)) {
+void launch_ring(unsigned grid, int threads, int64_t smem, int64_t fixed, cudaStream_t s, const NormParams& p) {
+    static std::atomic<int> allowed{-1};  // the device of the last call
+    if (smem + fixed > (48 << 10)) {
         int dev = 0;
         cudaGetDevice(&dev);
-        const int64_t want = static_cast<int64_t>(dev) << 32 | smem;
-        if (allowed.load(std::memory_order_relaxed) != want &&
+        if (allowed.load(std::memory_order_relaxed) != dev &&
             cudaFuncSetAttribute(kernel, cudaFuncAttributeMaxDynamicSharedMemorySize, static_cast<int>(smem)) == cudaSuccess)
-            allowed.store(want, std::memory_order_relaxed);
+            allowed.store(dev, std::memory_order_relaxed);
     }
     kernel<<<grid, threads, static_cast<size_t>(smem), s>>>(p);
 }
@@ -712,8 +715,11 @@ void forward_typed(NormParams p, int sms, cudaStream_t s) {
     const int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
     const int64_t blocks = T == 32 ? (p.rows + kWarpsPerBlock - 1) / kWarpsPerBlock : p.rows;
     const unsigned grid = static_cast<unsigned>(std::min<int64_t>(blocks, (T == 1024 ? 1ll : T == 256 ? 4ll : 2ll) * sms));
-    if (p.x_bf16) launch_ring<layer_norm_kernel<T, NE, G, true>>(grid, threads, smem, s, p);
-    else launch_ring<layer_norm_kernel<T, NE, G, false>>(grid, threads, smem, s, p);
+    if (p.x_bf16) {
+        launch_ring<layer_norm_kernel<T, NE, G, true>>(grid, threads, smem, kPartBytes, s, p);
+    } else {
+        if constexpr (G != 8) launch_ring<layer_norm_kernel<T, NE, G, false>>(grid, threads, smem, kPartBytes, s, p);
+    }
 }
 
 // group: the columns of 16 bytes of the call's widest type, or 1 where its rows do not allow 16-byte accesses.
@@ -729,15 +735,15 @@ void backward_typed(NormParams p, unsigned grid, cudaStream_t s) {
     constexpr int threads = T == 32 ? 32 * kWarpsPerBlock : T;
     const int64_t slot = slot_bytes(T * NE, p.x_bf16 != 0, G > 1) + slot_bytes(T * NE, p.dy_bf16 != 0, G > 1);
     p.depth = depth_of({T, NE}, slot);
-    int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
-    if (T == 32) smem = std::max<int64_t>(smem, 2 * kWarpsPerBlock * p.cols * static_cast<int64_t>(sizeof(float)));
-    if (p.x_bf16 && p.dy_bf16) launch_ring<layer_norm_backward_kernel<T, NE, G, true, true>>(grid, threads, smem, s, p);
-    else if (p.x_bf16) {
-        if constexpr (G != 8) launch_ring<layer_norm_backward_kernel<T, NE, G, true, false>>(grid, threads, smem, s, p);
-    } else if (p.dy_bf16) {
-        if constexpr (G != 8) launch_ring<layer_norm_backward_kernel<T, NE, G, false, true>>(grid, threads, smem, s, p);
-    } else {
-        if constexpr (G != 8) launch_ring<layer_norm_backward_kernel<T, NE, G, false, false>>(grid, threads, smem, s, p);
+    // (Two rows of at least 4 bytes a column for each warp: room for the warps' column sums at the end.)
+    const int64_t smem = p.depth * slot * (T == 32 ? kWarpsPerBlock : 1);
+    constexpr int64_t fixed = kPartBytes + (kSharedGain<NE> ? 4 * T * NE : 16 * T);
+    if (p.x_bf16 && p.dy_bf16) {
+        launch_ring<layer_norm_backward_kernel<T, NE, G, true, true>>(grid, threads, smem, fixed, s, p);
+    } else if constexpr (G != 8) {
+        if (p.x_bf16) launch_ring<layer_norm_backward_kernel<T, NE, G, true, false>>(grid, threads, smem, fixed, s, p);
+        else if (p.dy_bf16) launch_ring<layer_norm_backward_kernel<T, NE, G, false, true>>(grid, threads, smem, fixed, s, p);
+        else launch_ring<layer_norm_backward_kernel<T, NE, G, false, false>>(grid, threads, smem, fixed, s, p);
     }
 }
 
