@@ -649,7 +649,10 @@ __global__ void __launch_bounds__(256) layer_norm_wide_columns_kernel(const Norm
 // barrier, but past 1,024 columns (768 in the backward pass, which holds five values for each) its registers run out.
 // Blocks are as narrow as can hold the row: what binds them is the chain of barriers and reads of a row, so two blocks of
 // 256 threads on an SM, with a row each, beat one of 512 (backward pass of 3,001 x 5,003 bf16: 30 us, with 512 threads
-// 46 us, with 1,024 50 us).
+// 46 us, with 1,024 50 us). A thread has the fewest elements that hold the row, in fours: 12 against 16 for 5,001 rows of 2,999
+// columns, 41.2 against 45.3 us bf16 and 50.1 against 51.0 f32, 36.1 against 44.3 for 2,816 columns f32; 20 against 24, which
+// read the row twice, for 3,401 of 4,403, 37.2 against 40.8 bf16 and 46.6 against 58.7 f32 (whole calls). Eights of bf16 round
+// up to 16 and 24. Past 6,144 columns the five values a column (8,192), or the forward pass's three (16,384), are too many.
 struct Shape {
     int threads, elements;
 };
@@ -658,7 +661,7 @@ Shape shape_of(uint64_t cols, bool backward) {
     if (cols <= (backward ? 768 : 1024)) return {32, static_cast<int>((cols + 255) / 256) * 8};
     if (cols <= 1024) return {128, 8};
     if (cols <= 2048) return {256, 8};
-    if (backward && cols <= 6144) return {256, cols <= 4096 ? 16 : cols <= 5120 ? 20 : 24};
+    if (backward && cols <= 6144) return {256, static_cast<int>((cols + 1023) / 1024) * 4};
     if (cols <= 4096) return {512, 8};
     if (cols <= 6144) return {512, 12};
     if (cols <= 8192) return {512, 16};
@@ -847,6 +850,7 @@ int layer_norm_backward_launch(cudaStream_t s, const snb_layer_norm_args& a, std
         case 32 * 64 + 24: backward_shaped<32, 24>(p, group, grid, s); break;
         case 128 * 64 + 8: backward_shaped<128, 8>(p, group, grid, s); break;
         case 256 * 64 + 8: backward_shaped<256, 8>(p, group, grid, s); break;
+        case 256 * 64 + 12: backward_shaped<256, 12>(p, group, grid, s); break;
         case 256 * 64 + 16: backward_shaped<256, 16>(p, group, grid, s); break;
         case 256 * 64 + 20: backward_shaped<256, 20>(p, group, grid, s); break;
         case 256 * 64 + 24: backward_shaped<256, 24>(p, group, grid, s); break;
