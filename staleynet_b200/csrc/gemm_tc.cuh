@@ -731,7 +731,8 @@ __device__ __forceinline__ void softmax_grad_tile(const TcParams& p, const CUten
     const uint32_t target = live ? __ldg(p.targets + row) : kNoTarget;
     // 2^(k z - k max - log2 sum) in two steps: their sum in one f32 would round by up to 2^-24 of itself, a relative
     // error of that size times ln 2 in every value of the row.
-    const float2 stats = live ? __ldg(p.row_stats + row) : make_float2(0.0f, 0.0f);
+    // (An ordinary load: the kernel before this one writes the statistics, perhaps after this one has started.)
+    const float2 stats = live ? p.row_stats[row] : make_float2(0.0f, 0.0f);
     const float2 base = f2(-stats.x), rest = f2(-stats.y);
     const int64_t t64 = static_cast<int64_t>(target) - p.class_begin;
     const int32_t tcol = target != kNoTarget && t64 >= 0 && t64 < p.N ? static_cast<int32_t>(t64) : -1;

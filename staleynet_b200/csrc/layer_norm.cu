@@ -558,8 +558,9 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* s
     const float* src = sums + static_cast<int64_t>(blockIdx.y) * parts * cols;
     float s = 0.0f;
     if (c < cols) {
+        // (Ordinary loads: the sums are still being written when this kernel starts, which rules out the read-only path.)
 #pragma unroll 4
-        for (int64_t k = w; k < parts; k += 32) s += __ldg(src + k * cols + c);
+        for (int64_t k = w; k < parts; k += 32) s += src[k * cols + c];
     }
     part[w][lane] = s;
     __syncthreads();
