@@ -231,7 +231,7 @@ enum {
 };
 
 /* Caps, for the calling thread, the SMs that the persistent tensor-core GEMM grid of later snb_matmul,
- * snb_matmul_bf16 and snb_gemm calls may occupy (sms <= 0: all of them, the default). The GEMM kernels keep one CTA
+ * snb_matmul_bf16, snb_gemm and snb_vocabulary_cross_entropy calls may occupy (sms <= 0: all of them, the default). The GEMM kernels keep one CTA
  * (or CTA pair) per SM for the whole launch and assign work units to CTAs statically, so a kernel that holds some SMs
  * meanwhile (a collective on another stream) stretches every GEMM by a whole CTA's share of work; with a budget the
  * GEMM leaves those SMs free. Returns the previous setting. No reference counterpart. */
@@ -407,7 +407,7 @@ typedef struct snb_vocabulary_loss_args {
     const uint32_t* targets;   /* [rows]; 0xFFFFFFFF: the row has none (loss 0, zero gradient, whatever it holds);
                                 * any other value >= classes gives a NaN loss and gradient */
     uint64_t targets_len;
-    float* losses;             /* [rows] */
+    float* losses;             /* [rows], dense; never below 0 */
     uint64_t losses_len;
     float* loss_sum;           /* their sum, in a fixed order; or NULL */
     float grad_scale;
@@ -493,8 +493,9 @@ typedef struct snb_layer_norm_args {
 /* *bytes = the workspace of snb_layer_norm_backward on the current device. */
 SNB_API int snb_layer_norm_workspace(uint64_t rows, uint64_t cols, uint64_t* bytes);
 
-/* Checks of both, in this order: sizes, types and strides, "params length" (params_len != cols), lengths, null and
- * misaligned pointers, workspace. No reference counterpart (the reference normalises by the root mean square). */
+/* Checks of both, in this order: sizes, "params length" (params_len != cols), length of the statistics, null and misaligned
+ * parameters and statistics; then each tensor's type, stride, length and pointer; workspace. No reference counterpart (the
+ * reference normalises by the root mean square). */
 SNB_API int snb_layer_norm_forward(void* stream, const snb_layer_norm_args* args);
 
 /* input_grad, and the sums over the rows gain_grad and bias_grad, in a fixed order (the same from run to run). */

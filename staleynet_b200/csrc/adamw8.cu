@@ -210,7 +210,7 @@ __device__ __forceinline__ double block_sum(double v) {
 }
 
 // The sum of the squares of all gradients, a partial sum for each thread block. Bound by memory: 97.6 million f32 gradients
-// (391 MB, 60 us at the copy rate) take 77 us; 4.8 million bf16 ones, a latency, 6.3 us.
+// (391 MB, 60 us at the copy rate) take 77 us, bf16 ones (195 MB, 30 us) 42 us; 4.8 million bf16 ones, a latency, 6.3 us.
 __global__ void __launch_bounds__(32 * kWarps) adamw8_norm_kernel(const __grid_constant__ Table m, double* partials) {
     double sum = 0.0;
     for (Share s = share_of(m); s.part < s.end; next_tensor(m, s)) {
@@ -264,8 +264,8 @@ struct StepParams {
 
 // The step. A warp takes the 256 elements that share a scale, eight a lane, and holds them in registers from the read to the
 // code, since the new scale is known only when the last of them is. 97.6 million elements with f32 gradients and bf16 copies
-// (1.76 GB, 272 us at the copy rate) take 418 us, with the arithmetic and the memory traffic (348 us alone) overlapping for
-// the most part; three resident blocks an SM at 80 registers, against 469 us for two. 4.8 million elements with bf16
+// (1.76 GB, 272 us at the copy rate) take 407 to 418 us, with the arithmetic and the memory traffic (348 us alone) overlapping
+// for the most part, and with bf16 gradients (1.56 GB, 242 us) 409 us; three resident blocks an SM at 80 registers, against 469 us for two. 4.8 million elements with bf16
 // gradients (76 MB): 28 us, bound by the latency of five passes of a warp.
 __global__ void __launch_bounds__(32 * kWarps, kStepBlocks) adamw8_step_kernel(const __grid_constant__ Table m, const StepParams a) {
     // Every thread block adds the norm's partial sums in the same order.

@@ -283,7 +283,8 @@ struct NormParams {
 // Both kernels: T threads a row, NE elements a thread, `depth` rows in flight in shared memory (a ring for each warp when
 // T is 32, else one of the block), rows first, first + step, ... . kMaxDepth bounds the waits' immediate operands.
 //
-// Measured. Forward, 65,536 x 768 bf16 (202 MB, 31 us at the copy rate): 33 us; one row of 768 f32: 2.4 us, a launch.
+// Measured. Forward, 65,536 x 768 bf16 (202 MB, 31 us at the copy rate): 33 us; f32 (403 MB, 62 us): 73 us a call, backward
+// 105 us (605 MB, 94 us); one row of 768 f32: 2.4 us, a launch.
 // Backward, 65,536 x 768 bf16 (302 MB, 47 us at the copy rate): 51 us; 4,096 x 256 f32: 4.1 us; 3,001 x 5,003 bf16, whose
 // rows start off every boundary (90 MB, 14 us): 29 us, bound by the chain of each row, which two barriers interrupt, and by
 // its single-element reads from shared memory.
@@ -571,7 +572,8 @@ __global__ void __launch_bounds__(1024) layer_norm_columns_kernel(const float* s
 }
 
 // Rows of any length, a block each, read three times (forward) or twice (backward). What binds them is those passes, which
-// mostly hit L1 and L2; they stand for rows that the shapes below have no registers for.
+// mostly hit L1 and L2, element by element; they stand for rows that the shapes below have no registers for. Backward pass of
+// 4,096 x 9,001 bf16: 224 us (221 MB, 34 us at the copy rate); of 4,096 x 12,288: 309 us (302 MB, 47 us).
 constexpr int kWideThreads = 512;
 
 __device__ __forceinline__ float element(const void* row, int64_t c, bool bf16) {

@@ -513,7 +513,8 @@ bool aligned16(const void* p) { return reinterpret_cast<uintptr_t>(p) % 16 == 0;
 
 // Whether the few rows' kernels take a call: the loss alone of hidden rows that fit into shared memory as f32 (64 KB for
 // four), where the tensor cores would need a packed copy of the weight first. Measured over 100,000 x 1,024 f32 (63 us at
-// the copy rate): 1 row 90 us, 4 rows 100 us, 5 rows by way of the split copy 634 us, so f32 goes up to 16 rows, four a
+// the copy rate): 1 row 90 us, 4 rows 100 us, 16 rows 388 us (weight [classes, width]) or 578 us, by way of the split copy 5
+// to 17 rows 592 to 634 us, so f32 goes up to 16 rows, four a
 // pass; over 512 x 50,021 bf16, whose rows lie off every boundary: 1 row 48 us, 4 rows 53 us, packed 62 us. A bf16 weight
 // that TMA can read stays with the tensor cores (32,000 x 768: 1 row 23 us here, 19 us there).
 bool few_rows(const snb_vocabulary_loss_args& a) {
@@ -539,6 +540,7 @@ Layout layout_of(const snb_vocabulary_loss_args& a, int sms) {
     // (The hidden gradient's product has `seg` columns: those past the width must be zeros of a packed weight.)
     l.pack_weight = !l.few && (l.f32 || !aligned16(a.weight) || a.weight_stride % per16 != 0 ||
                                (a.hidden_grad != nullptr && a.width != l.seg));
+    // (Fitted to the whole device, whatever the budget of SMs, so that the workspace does not depend on that.)
     // A piece is as long as the bounds allow for P [rows, piece] and for the packed weight, in whole tiles: long pieces
     // make long sums for the hidden gradient and few additions into it. Between half that length and all of it, the one is
     // taken whose weight gradient fills the last round of CTA pairs best (measured at 16,384 x 768 x 131,072: pieces of
